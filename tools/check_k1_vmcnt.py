@@ -116,7 +116,8 @@ def main():
         path = sys.argv[1]
     else:
         path = os.path.join(tempfile.mkdtemp(), "k1.s")
-        subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "-O3", "-std=c++17", "--offload-arch=gfx950", "-S",
+        subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "-O3", "-std=c++17", "--offload-arch=gfx950",
+                        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-S",
                         "--cuda-device-only", "-o", path, os.path.join(ROOT, "dp_timeautodiff_amd/csrc/k1_linear_gs.hip")],
                        check=True, stderr=subprocess.DEVNULL)
     kernels, cur, name = {}, None, None
