@@ -60,6 +60,25 @@ EXPORTS = {
     "dpk_gru_pack_backward": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "dpk_gru_forward": (c_int, [c_void_p] * 12 + [c_int, c_int, c_int, c_int, c_void_p]),
     "dpk_gru_backward": (c_int, [c_void_p] * 10 + [c_int, c_int, c_int, c_int, c_void_p]),
+    "dpk_rms_norm_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_int64, c_int, c_float, c_int, c_void_p]),
+    "dpk_rms_norm_split": (c_int, [c_int64, c_int64]),
+    "dpk_rms_norm_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]),
+    "dpk_causal_conv_segments": (c_int, [c_int, c_int, c_int]),
+    "dpk_causal_conv_forward": (c_int, [c_void_p, c_int64, c_int64] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
+    "dpk_causal_conv_backward": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 8
+                                 + [c_int64, c_int64] + [c_int] * 6 + [c_float, c_int, c_int, c_void_p]),
+    "dpk_causal_conv_step": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "dpk_selective_scan_chunks": (c_int, [c_int, c_int, c_int, c_void_p]),
+    "dpk_selective_scan_group": (c_int, []),
+    "dpk_selective_scan_channel_blocks": (c_int, [c_int]),
+    "dpk_selective_scan_forward": (c_int, [c_void_p] * 4),
+    "dpk_selective_scan_backward": (c_int, [c_void_p] * 3),
+    "dpk_selective_scan_step": (c_int, [c_void_p] * 4),
+    "dpk_compress_activation": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
+    "dpk_restore_activation": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
+    "dpk_sum_rows": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_int64, c_float, c_int, c_void_p]),
 }
 
 
@@ -637,3 +656,433 @@ def poisson_sample(seed: int, offset: int, sample_rate: float, N: int, idx: torc
     rc = load().dpk_poisson_sample(seed & (2**64 - 1), offset & (2**64 - 1), _ptr(offset_dev), float(sample_rate),
                                    int(N), idx.numel(), _ptr(idx), _ptr(counts), _stream())
     _check(rc, "dpk_poisson_sample")
+
+
+# ---- K12..K15: the state-space layer ------------------------------------------------------------------------------
+# Activations are fp32, bf16 or fp16; parameters, scan states and parameter gradients are fp32.  Every call runs on the
+# current stream of its tensors' device, whichever device is current.
+
+ACT_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+RMS_MAX_FEATURES = 16384
+CONV_MAX_WIDTH = 4
+SCAN_MAX_STATE = 32
+ACT8_BLOCK = 128
+
+
+def _act(t, name: str, shape=None, like: Optional[torch.Tensor] = None):
+    """An activation: HIP tensor of an activation dtype, of `shape`, with `like`'s dtype and device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise DpkError(f"{name}: expected a CUDA/HIP tensor (this package has no CPU path)")
+    if t.dtype not in ACT_DTYPES:
+        raise DpkError(f"{name}: expected fp32, bf16 or fp16, got {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise DpkError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise DpkError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _par(t, name: str, shape, device, dtype=torch.float32):
+    """A parameter, state or index vector: dense, of one shape, on the activations' device."""
+    if t is None:
+        return None
+    _req(t, name, dtype)
+    if tuple(t.shape) != tuple(shape) or t.device != device:
+        raise DpkError(f"{name}: expected shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+class _on:
+    """Makes the tensors' device current for a launch and yields the stream argument."""
+    __slots__ = ("device", "guard")
+
+    def __init__(self, device):
+        self.device, self.guard = device, None
+
+    def __enter__(self):
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _as_rows(t: torch.Tensor):
+    """(tensor, row stride) of [..., C] seen as rows of one stride; copied only if the layout has none."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    if t.stride(-1) == 1 and (t.dim() == 2 or (t.dim() == 3 and t.stride(0) == t.shape[1] * t.stride(1))):
+        return t, t.stride(-2)
+    return t.contiguous(), t.shape[-1]
+
+
+def _as_btf(t: torch.Tensor):
+    """[B, T, F] whose last dimension is contiguous."""
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def sum_rows(src: torch.Tensor, groups: int, rows: int, P: int, in_stride: int, out_ptr, out_stride: int, scale: float,
+             accumulate: bool, stream):
+    _check(load().dpk_sum_rows(src if isinstance(src, c_void_p) else _ptr(src), groups, rows, P, in_stride, out_ptr, out_stride,
+                               float(scale), int(accumulate), stream), "dpk_sum_rows")
+
+
+def rms_norm_forward(x, residual, weight, eps: float, want_rstd: bool, quantize: bool):
+    """Returns y, r (None without a residual), rstd [rows] (or None), q int8 and exponent bytes (or None, None)."""
+    _act(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise DpkError("x: expected [..., C] with C > 0")
+    C = x.shape[-1]
+    if C > RMS_MAX_FEATURES:
+        raise DpkError(f"rms_norm: at most {RMS_MAX_FEATURES} features, got {C}")
+    if not eps >= 0:
+        raise DpkError(f"rms_norm: eps must not be negative, got {eps}")
+    weight = _par(weight, "weight", (C,), x.device)
+    if weight is None:
+        raise DpkError("rms_norm: weight is None")
+    x, ld_x = _as_rows(x)
+    ld_res = 0
+    if residual is not None:
+        _act(residual, "residual", x.shape, x)
+        residual, ld_res = _as_rows(residual)
+    rows = x.numel() // C
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    r = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
+    q = e = None
+    if quantize:
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        e = torch.empty(*x.shape[:-1], -(-C // ACT8_BLOCK), dtype=torch.uint8, device=x.device)
+    if rows:
+        with _on(x.device) as stream:
+            _check(load().dpk_rms_norm_forward(_ptr(x), ld_x, _ptr(residual), ld_res, _ptr(weight), _ptr(y), _ptr(r), _ptr(rstd),
+                                               _ptr(q), _ptr(e), rows, C, float(eps), ACT_DTYPES[x.dtype], stream),
+                   "dpk_rms_norm_forward")
+    return y, r, rstd, q, e
+
+
+def rms_norm_backward(r, dy, dr, weight, rstd, want_dx: bool, want_dw: bool, window: Optional[FlatView] = None,
+                      scale: float = 1.0, accumulate: bool = False):
+    """r, dy, dr (None = zeros) [..., C].  Returns dx (or None) and the weight's gradient: [C] summed over all rows, or None with
+    `window` given: then row b of the window receives (or is added) `scale` times the gradient of sample b = r[b]."""
+    C = r.shape[-1]
+    rows = r.numel() // C
+    groups = r.shape[0] if window is not None else 1
+    r, ld_r = _as_rows(r)
+    dy, ld_dy = _as_rows(dy)
+    ld_dr = 0
+    if dr is not None:
+        dr, ld_dr = _as_rows(dr)
+    dev = r.device
+    dx = torch.empty(r.shape, dtype=r.dtype, device=dev) if want_dx else None
+    if window is not None and (window.numel != C or window.base.shape[0] < groups):
+        raise DpkError("rms_norm: grad-sample window does not match the layer")
+    dw = torch.empty(C, dtype=torch.float32, device=dev) if want_dw and window is None else None
+    if window is not None and groups == 0:
+        return dx, None
+    lib = load()
+    per = rows // groups
+    split = lib.dpk_rms_norm_split(groups, per)
+    ws = torch.empty(groups * split, C, dtype=torch.float32, device=dev) if split > 1 and want_dw else None
+    with _on(dev) as stream:
+        if window is not None:
+            out, stride = window.ptr, window.stride
+        else:
+            out, stride = _ptr(dw), C
+        direct = ws is None
+        _check(lib.dpk_rms_norm_backward(_ptr(r), ld_r, _ptr(dy), ld_dy, _ptr(dr), ld_dr, _ptr(weight), _ptr(rstd), _ptr(dx),
+                                         (out if direct else _ptr(ws)) if want_dw else None, stride if direct else C, groups, per,
+                                         split, C, float(scale) if direct else 1.0, int(accumulate and direct),
+                                         ACT_DTYPES[r.dtype], stream), "dpk_rms_norm_backward")
+        if not direct:
+            sum_rows(ws, groups, split, C, C, out, stride, scale, accumulate, stream)
+    return dx, dw
+
+
+def _conv_args(x, weight, bias, state, lengths):
+    _act(x, "x")
+    if x.dim() != 3 or x.shape[2] == 0:
+        raise DpkError(f"causal_conv: x must be [B, T, D] with D > 0, got {tuple(x.shape)}")
+    B, T, D = x.shape
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= CONV_MAX_WIDTH:
+        raise DpkError(f"causal_conv: weight must be [D, W] with W of 1 to {CONV_MAX_WIDTH}")
+    W = weight.shape[1]
+    weight = _par(weight, "weight", (D, W), x.device)
+    bias = _par(bias, "bias", (D,), x.device)
+    if state is not None:
+        _act(state, "state", (B, W - 1, D), x)
+        state = state.contiguous()
+    lengths = _par(lengths, "lengths", (B,), x.device, torch.int32)
+    return _as_btf(x), weight, bias, state, lengths, W
+
+
+def causal_conv_forward(x, weight, bias, state, lengths, silu: bool, want_state: bool):
+    """Returns y [B,T,D] and the state behind each sequence [B,W-1,D] (or None)."""
+    x, weight, bias, state, lengths, W = _conv_args(x, weight, bias, state, lengths)
+    B, T, D = x.shape
+    y = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
+    out = torch.empty(B, W - 1, D, dtype=x.dtype, device=x.device) if want_state else None
+    if B:
+        with _on(x.device) as stream:
+            _check(load().dpk_causal_conv_forward(_ptr(x), x.stride(0), x.stride(1), _ptr(weight), _ptr(bias), _ptr(state),
+                                                  _ptr(lengths), _ptr(y), _ptr(out), B, T, D, W, int(silu),
+                                                  ACT_DTYPES[x.dtype], stream), "dpk_causal_conv_forward")
+    return y, out
+
+
+def causal_conv_backward(x, weight, bias, state, lengths, silu: bool, dy, dstate_out, want_dstate: bool, want_par: bool,
+                         windows=None, scale: float = 1.0, accumulate: bool = False):
+    """Returns dx, dstate (or None) and the parameters' gradients: (dw [D,W], db [D] or None) summed over the batch, or None
+    with `windows` = (weight window, bias window or None): then their rows receive the per-sample gradients."""
+    x, weight, bias, state, lengths, W = _conv_args(x, weight, bias, state, lengths)
+    B, T, D = x.shape
+    _act(dy, "dy", x.shape, x)
+    dy = _as_btf(dy)
+    if dstate_out is not None:
+        _act(dstate_out, "dstate", (B, W - 1, D), x)
+        dstate_out = dstate_out.contiguous()
+    dev = x.device
+    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
+    dstate = torch.empty(B, W - 1, D, dtype=x.dtype, device=dev) if want_dstate else None
+    nb = 0 if bias is None else D
+    flat = torch.empty(D * W + nb, dtype=torch.float32, device=dev) if want_par and windows is None else None
+    lib = load()
+    seg = lib.dpk_causal_conv_segments(B, T, D)
+    ww, wb = windows if windows is not None else (None, None)
+    if ww is not None and (ww.numel != D * W or ww.base.shape[0] < B or (wb is None) != (bias is None)
+                           or (wb is not None and wb.numel != D)):
+        raise DpkError("causal_conv: grad-sample windows do not match the layer")
+    direct = ww is not None and seg == 1   # one segment: the kernel's row is the sample's arena row
+    if direct:
+        par, stride, off = ww.ptr, ww.stride, (wb.offset - ww.offset if wb is not None else -1)
+        direct = wb is None or off >= 0
+    ws = None
+    if want_par and not direct:
+        ws = torch.empty(max(B * seg, 1), D * W + nb, dtype=torch.float32, device=dev)
+        par, stride, off = _ptr(ws), D * W + nb, (D * W if nb else -1)
+    with _on(dev) as stream:
+        if B:
+            _check(lib.dpk_causal_conv_backward(
+                _ptr(x), x.stride(0), x.stride(1), _ptr(dy), dy.stride(0), dy.stride(1), _ptr(weight), _ptr(bias), _ptr(state),
+                _ptr(dstate_out), _ptr(lengths), _ptr(dx), _ptr(dstate), par if want_par else None, stride if want_par else 0,
+                off if want_par else -1, seg, B, T, D, W, int(silu), float(scale) if direct else 1.0, int(accumulate and direct),
+                ACT_DTYPES[x.dtype], stream), "dpk_causal_conv_backward")
+        if flat is not None:
+            sum_rows(ws, 1, B * seg, D * W + nb, D * W + nb, _ptr(flat), D * W + nb, scale, False, stream)
+        elif ws is not None and B:
+            sum_rows(ws, B, seg, D * W, stride, ww.ptr, ww.stride, scale, accumulate, stream)
+            if wb is not None:
+                sum_rows(c_void_p(ws.data_ptr() + 4 * D * W), B, seg, D, stride, wb.ptr, wb.stride, scale, accumulate, stream)
+    grads = None if flat is None else (flat[:D * W].view(D, W), flat[D * W:] if nb else None)
+    return dx, dstate, grads
+
+
+def causal_conv_step(x, state, weight, bias, silu: bool):
+    """One token: x [B,D], state [B,W-1,D] updated in place.  Returns y [B,D]."""
+    _act(x, "x")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise DpkError(f"causal_conv_step: x must be [B, D] with D > 0, got {tuple(x.shape)}")
+    B, D = x.shape
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= CONV_MAX_WIDTH:
+        raise DpkError(f"causal_conv_step: weight must be [D, W] with W of 1 to {CONV_MAX_WIDTH}")
+    W = weight.shape[1]
+    weight = _par(weight, "weight", (D, W), x.device)
+    bias = _par(bias, "bias", (D,), x.device)
+    _act(state, "state", (B, W - 1, D), x)
+    if not state.is_contiguous():
+        raise DpkError("causal_conv_step: the state is updated in place and must be contiguous")
+    if x.stride(1) != 1 and D > 1:
+        x = x.contiguous()
+    y = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    if B:
+        with _on(x.device) as stream:
+            _check(load().dpk_causal_conv_step(_ptr(x), x.stride(0), _ptr(state), _ptr(weight), _ptr(bias), _ptr(y), B, D, W,
+                                               int(silu), ACT_DTYPES[x.dtype], stream), "dpk_causal_conv_step")
+    return y
+
+
+class _ScanDesc(ctypes.Structure):  # dpk_scan_desc (include/dpk.h)
+    _fields_ = ([(n, c_void_p) for n in ("u", "delta", "Bm", "Cm", "z", "A_log", "Dskip", "dt_bias", "h0", "lengths", "kept",
+                                         "edge", "span")]
+                + [(n, c_int64) for n in ("u_sb", "u_st", "delta_sb", "delta_st", "B_sb", "B_st", "C_sb", "C_st", "z_sb", "z_st")]
+                + [(n, c_int) for n in ("B", "T", "D", "N", "softplus", "nchunk", "chunk", "dtype")])
+
+
+class _ScanGrads(ctypes.Structure):  # dpk_scan_grads (include/dpk.h)
+    _fields_ = ([(n, c_void_p) for n in ("dout", "dhT", "du", "ddelta", "dB", "dC", "dz", "dh0", "dbc", "dA", "dD", "dbias")]
+                + [(n, c_int64) for n in ("dout_sb", "dout_st", "par_stride")] + [("scale", c_float), ("accumulate", c_int)])
+
+
+class ScanInputs:
+    """The checked operands of a selective scan, laid out as the kernels read them."""
+    __slots__ = ("u", "delta", "A_log", "B", "C", "D", "z", "dt_bias", "h0", "lengths", "softplus")
+
+    def __init__(self, u, delta, A_log, B, C, D, z, dt_bias, h0, lengths, softplus, step: bool = False):
+        _act(u, "u")
+        lead = 2 if step else 3
+        if u.dim() != lead or u.shape[-1] == 0:
+            raise DpkError(f"selective_scan: u must be {'[B, D]' if step else '[B, T, D]'} with D > 0, got {tuple(u.shape)}")
+        if not isinstance(A_log, torch.Tensor) or A_log.dim() != 2 or not 1 <= A_log.shape[1] <= SCAN_MAX_STATE:
+            raise DpkError(f"selective_scan: A_log must be [D, N] with N of 1 to {SCAN_MAX_STATE}")
+        d, n = u.shape[-1], A_log.shape[1]
+        rows = tuple(u.shape[:-1])
+        _act(delta, "delta", u.shape, u)
+        for t, name in ((B, "B"), (C, "C")):
+            _act(t, name, rows + (n,), u)
+        if z is not None:
+            _act(z, "z", u.shape, u)
+        dense = (lambda t: t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous())
+        self.u, self.delta, self.B, self.C, self.z = (dense(t) for t in (u, delta, B, C, z))
+        dev = u.device
+        self.A_log = _par(A_log, "A_log", (d, n), dev)
+        self.D = _par(D, "D", (d,), dev)
+        self.dt_bias = _par(dt_bias, "dt_bias", (d,), dev)
+        self.h0 = _par(h0, "state", (u.shape[0], d, n), dev)
+        self.lengths = _par(lengths, "lengths", (u.shape[0],), dev, torch.int32)
+        self.softplus = bool(softplus)
+
+    def desc(self, kept=None):
+        """dpk_scan_desc and the scratch it points at."""
+        u = self.u
+        b, t = (u.shape[0], u.shape[1]) if u.dim() == 3 else (u.shape[0], 1)
+        d, n = self.A_log.shape
+        chunk = c_int(0)
+        nchunk = load().dpk_selective_scan_chunks(b, t, d, ctypes.byref(chunk)) if u.dim() == 3 else 1
+        s = _ScanDesc()
+        s.B, s.T, s.D, s.N, s.softplus, s.dtype = b, t, d, n, int(self.softplus), ACT_DTYPES[u.dtype]
+        s.nchunk, s.chunk = nchunk, chunk.value if u.dim() == 3 else load().dpk_selective_scan_group()
+        for name, x in (("u", u), ("delta", self.delta), ("Bm", self.B), ("Cm", self.C), ("z", self.z), ("A_log", self.A_log),
+                        ("Dskip", self.D), ("dt_bias", self.dt_bias), ("h0", self.h0), ("lengths", self.lengths), ("kept", kept)):
+            setattr(s, name, None if x is None else x.data_ptr())
+        for name, x in (("u", u), ("delta", self.delta), ("B", self.B), ("C", self.C), ("z", self.z)):
+            if x is not None:
+                setattr(s, name + "_sb", x.stride(0))
+                setattr(s, name + "_st", x.stride(1) if x.dim() == 3 else 0)
+        scratch = None
+        if nchunk > 1:
+            scratch = torch.empty(nchunk * b * (n + 1) * d, dtype=torch.float32, device=u.device)
+            s.edge = scratch.data_ptr()
+            s.span = scratch.data_ptr() + 4 * nchunk * b * n * d
+        return s, scratch
+
+
+def selective_scan_forward(inp: ScanInputs, want_kept: bool, want_state: bool):
+    """Returns out [B,T,D], the final state [B,D,N] (or None) and the states kept for the backward pass (or None)."""
+    u = inp.u
+    b, t, d = u.shape
+    n = inp.A_log.shape[1]
+    lib = load()
+    out = torch.empty(b, t, d, dtype=u.dtype, device=u.device)
+    hT = torch.empty(b, d, n, dtype=torch.float32, device=u.device) if want_state else None
+    g = lib.dpk_selective_scan_group()
+    kept = torch.empty(b, (t + g - 1) // g, n, d, dtype=torch.float32, device=u.device) if want_kept else None
+    if b:
+        with _on(u.device) as stream:
+            s, scratch = inp.desc(kept)
+            _check(lib.dpk_selective_scan_forward(ctypes.byref(s), _ptr(out), _ptr(hT), stream), "dpk_selective_scan_forward")
+    return out, hT, kept
+
+
+def selective_scan_backward(inp: ScanInputs, kept, dout, dhT, want_dh0: bool, want_par: bool, windows=None, scale: float = 1.0,
+                            accumulate: bool = False):
+    """Returns du, ddelta, dB, dC, dz (or None), dh0 (or None) and the parameters' gradients: (dA_log [D,N], dD [D], ddt_bias [D])
+    summed over the batch, or None with `windows` = arena windows of (A_log, D, dt_bias) (the latter two may be None)."""
+    u = inp.u
+    b, t, d = u.shape
+    n = inp.A_log.shape[1]
+    dev = u.device
+    _act(dout, "dout", u.shape, u)
+    dout = dout if dout.stride(2) == 1 or d == 1 else dout.contiguous()
+    dhT = _par(dhT, "dstate", (b, d, n), dev)
+    new = lambda *shape: torch.empty(*shape, dtype=u.dtype, device=dev)  # noqa: E731
+    du, ddelta, dB, dC = new(b, t, d), new(b, t, d), new(b, t, n), new(b, t, n)
+    dz = new(b, t, d) if inp.z is not None else None
+    dh0 = torch.empty(b, d, n, dtype=torch.float32, device=dev) if want_dh0 else None
+    P = d * (n + 2)
+    flat = torch.empty(P, dtype=torch.float32, device=dev) if want_par and windows is None else None
+    if windows is not None:
+        for w, size in zip(windows, (d * n, d, d)):
+            if w is not None and (w.numel != size or w.base.shape[0] < b):
+                raise DpkError("selective_scan: grad-sample windows do not match the layer")
+    lib = load()
+    if b:
+        with _on(dev) as stream:
+            s, scratch = inp.desc(kept)
+            g = _ScanGrads()
+            g.dout, g.dout_sb, g.dout_st = dout.data_ptr(), dout.stride(0), dout.stride(1)
+            for name, x in (("dhT", dhT), ("du", du), ("ddelta", ddelta), ("dB", dB), ("dC", dC), ("dz", dz), ("dh0", dh0)):
+                setattr(g, name, None if x is None else x.data_ptr())
+            blocks = lib.dpk_selective_scan_channel_blocks(d)
+            dbc = torch.empty(blocks, b, t, 2 * n, dtype=torch.float32, device=dev) if blocks > 1 else None
+            g.dbc = None if dbc is None else dbc.data_ptr()
+            direct = windows is not None and s.nchunk == 1
+            ws = None
+            g.scale, g.accumulate = 1.0, 0
+            if want_par and direct:
+                g.dA, g.dD, g.dbias = (None if w is None else w.ptr.value for w in windows)
+                g.par_stride, g.scale, g.accumulate = windows[0].stride, float(scale), int(accumulate)
+            elif want_par:
+                ws = torch.empty(b * s.nchunk, P, dtype=torch.float32, device=dev)
+                g.dA, g.dD, g.dbias = ws.data_ptr(), ws.data_ptr() + 4 * d * n, ws.data_ptr() + 4 * d * (n + 1)
+                g.par_stride = P
+            _check(lib.dpk_selective_scan_backward(ctypes.byref(s), ctypes.byref(g), stream), "dpk_selective_scan_backward")
+            if flat is not None:
+                sum_rows(ws, 1, b * s.nchunk, P, P, _ptr(flat), P, scale, False, stream)
+            elif ws is not None:
+                for w, off, size in zip(windows, (0, d * n, d * (n + 1)), (d * n, d, d)):
+                    if w is not None:
+                        sum_rows(c_void_p(ws.data_ptr() + 4 * off), b, s.nchunk, size, P, w.ptr, w.stride, scale, accumulate, stream)
+    elif flat is not None:
+        flat.zero_()
+    grads = None if flat is None else (flat[:d * n].view(d, n), flat[d * n:d * (n + 1)], flat[d * (n + 1):])
+    return du, ddelta, dB, dC, dz, dh0, grads
+
+
+def selective_scan_step(inp: ScanInputs, state):
+    """One token: operands [B,D] / [B,N], state [B,D,N] updated in place.  Returns out [B,D]."""
+    u = inp.u
+    b, d = u.shape
+    if state is None or _par(state, "state", (b, d, inp.A_log.shape[1]), u.device) is not state:
+        raise DpkError("selective_scan_step: the state is updated in place and must be a contiguous [B, D, N]")
+    out = torch.empty(b, d, dtype=u.dtype, device=u.device)
+    if b:
+        with _on(u.device) as stream:
+            s, _ = inp.desc()
+            _check(load().dpk_selective_scan_step(ctypes.byref(s), _ptr(state), _ptr(out), stream), "dpk_selective_scan_step")
+    return out
+
+
+def compress_activation(x):
+    """Returns q int8 (x's shape) and the exponent bytes [..., ceil(C/128)]."""
+    _act(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise DpkError("compress_activation: expected [..., C] with C > 0")
+    C = x.shape[-1]
+    x, ld = _as_rows(x)
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    e = torch.empty(*x.shape[:-1], -(-C // ACT8_BLOCK), dtype=torch.uint8, device=x.device)
+    if x.numel():
+        with _on(x.device) as stream:
+            _check(load().dpk_compress_activation(_ptr(x), ld, _ptr(q), _ptr(e), x.numel() // C, C, ACT_DTYPES[x.dtype], stream),
+                   "dpk_compress_activation")
+    return q, e
+
+
+def restore_activation(q, e, dtype):
+    _req(q, "data", torch.int8); _req(e, "exponent", torch.uint8)
+    if dtype not in ACT_DTYPES:
+        raise DpkError(f"restore_activation: expected fp32, bf16 or fp16, got {dtype}")
+    C = q.shape[-1]
+    if tuple(e.shape) != tuple(q.shape[:-1]) + (-(-C // ACT8_BLOCK),) or e.device != q.device:
+        raise DpkError("restore_activation: data and exponents do not belong together")
+    if not q.is_contiguous() or not e.is_contiguous():
+        raise DpkError("restore_activation: data and exponents must be contiguous")
+    x = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if q.numel():
+        with _on(q.device) as stream:
+            _check(load().dpk_restore_activation(_ptr(q), _ptr(e), _ptr(x), q.numel() // C, C, ACT_DTYPES[dtype], stream),
+                   "dpk_restore_activation")
+    return x

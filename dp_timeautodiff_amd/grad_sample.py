@@ -29,7 +29,8 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .layers import RNNLinear, SequenceBias
+from .activation8 import Activation8, compress_activation, restore_activation
+from .layers import DPCausalConv, DPRMSNorm, DPSelectiveScan, RNNLinear, SequenceBias, SSMLinear
 from .layers.fused_gru import FusedLinearCellGRU
 
 ARENA_ALIGN = 64  # floats: every parameter window starts on a 256-byte boundary
@@ -177,11 +178,12 @@ class _Layer:
         self.pairs: List[Tuple[torch.Tensor, torch.Tensor]] = []
         self.counter = 0
         self.passes_written = 0
+        self.open_task = None  # kind "own": autograd graph task of the backward pass whose rows are being written
 
 
 def _kind_of(m: nn.Module) -> Optional[str]:
     t = type(m)
-    if t in (nn.Linear, RNNLinear):
+    if t in (nn.Linear, RNNLinear, SSMLinear):
         return "linear"
     if t is nn.Embedding:
         return "embedding"
@@ -189,7 +191,73 @@ def _kind_of(m: nn.Module) -> Optional[str]:
         return "layernorm"
     if t is SequenceBias:
         return "seqbias"
+    if issubclass(t, (DPRMSNorm, DPCausalConv, DPSelectiveScan)):
+        return "own"  # the layer's backward kernel writes the per-sample gradients itself
     return None
+
+
+class _ArenaRows:
+    """Context of one backward kernel that writes its layer's per-sample gradients itself: the arena windows to write to, the
+    factor for them, and whether to add (the layer's second call within one backward pass).  Leaving it emits the norms."""
+
+    def __init__(self, gsm, layer, B):
+        self._gsm, self._layer, self._B = gsm, layer, B
+
+    def __enter__(self):
+        gsm, layer, B = self._gsm, self._layer, self._B
+        task = gsm._graph_task()
+        self.accumulate = task != -1 and task == layer.open_task
+        if self.accumulate:
+            if gsm.arena.pass_B[layer.passes_written - 1] != B:
+                raise NotImplementedError("a layer was called with different batch sizes within one forward pass")
+            self._k, self._row0 = layer.passes_written - 1, sum(gsm.arena.pass_B[:layer.passes_written - 1])
+        else:
+            self._k, self._row0 = gsm._claim_rows(layer, B)
+            layer.open_task = task
+        self.scale = float(B) if gsm.loss_reduction == "mean" else 1.0
+        return self
+
+    def window(self, name):
+        return self._gsm.arena.flat(getattr(self._layer.module, name), self._row0)
+
+    def __exit__(self, kind, *_):
+        if kind is not None:
+            return False
+        gsm, layer, arena = self._gsm, self._layer, self._gsm.arena
+        if self._B:
+            part, slot = (arena.part[self._row0:] if self._row0 else arena.part), layer.slot0
+            for p in layer.params:
+                w = arena.flat(p, self._row0)
+                _native.normsq_partials(w, self._B, part, slot)
+                slot += _native.normsq_slots(w.numel)
+        if not self.accumulate:
+            gsm._publish(layer.module, arena, self._row0, self._B, self._k)
+        return False
+
+
+class _Claim:
+    """What GradSampleModule hands a layer of kind "own"."""
+
+    def __init__(self, gsm, layer):
+        self._gsm, self._layer = gsm, layer
+
+    def sink(self, B):
+        return _ArenaRows(self._gsm, self._layer, B)
+
+    def enabled(self):
+        return self._gsm.hooks_enabled
+
+    @property
+    def anchor(self):
+        return self._gsm._tap_on(self._layer.params[0].device)
+
+    @property
+    def batch_first(self):
+        return self._gsm.batch_first
+
+    @property
+    def activation_bits(self):
+        return self._gsm.activation_bits
 
 
 class _GradTap(torch.autograd.Function):
@@ -210,8 +278,14 @@ class GradSampleModule(nn.Module):
 
     def __init__(self, m: nn.Module, *, batch_first: bool = True, loss_reduction: str = "mean",
                  strict: bool = True, force_functorch: bool = False, skip_autograd_param_grads: bool = True,
-                 overlap_grad_sample: bool = False):
+                 overlap_grad_sample: bool = False, activation_bits: int = 32):
         super().__init__()
+        # activation_bits=8: the inputs of Linear layers are stashed in 8 bits until the backward pass contracts them (a quarter of
+        # the memory, wherever nothing else holds the fp32 tensor; per-sample gradients carry the rounding of at most
+        # max|block of 128| / 127)
+        if activation_bits not in (8, 32):
+            raise ValueError(f"activation_bits = {activation_bits}. Only 8 and 32 are supported")
+        self.activation_bits = activation_bits
         # Autograd's own (summed) parameter gradients are never used by DP-SGD: DPOptimizer overwrites p.grad.
         # While a sampled layer runs forward on an input that already requires grad, its parameters are
         # switched to requires_grad=False, so backward computes only dL/dx (which the hooks need) and skips the
@@ -261,6 +335,8 @@ class GradSampleModule(nn.Module):
                 n = _native.linear_slots(sub.in_features, sub.out_features)
             elif kind == "seqbias":
                 n = _native.linear_slots(1, sub.bias.numel())
+            elif kind == "own":
+                n = sum(_native.normsq_slots(self.arena.window(p).numel) for p in own)
             elif kind == "layernorm":
                 if len(sub.normalized_shape) != 1 or not sub.elementwise_affine:
                     raise NotImplementedError(f"{name}: only affine LayerNorm over the last dim is supported")
@@ -275,6 +351,9 @@ class GradSampleModule(nn.Module):
             self._layers.append(layer)
             for p in own:
                 covered.add(id(p))
+            if kind == "own":
+                object.__setattr__(sub, "_dpk_claim", _Claim(self, layer))
+                continue
             self._handles.append(sub.register_forward_pre_hook(self._make_pre(layer)))
             self._handles.append(sub.register_forward_hook(self._make_fwd(layer)))
             self._handles.append(sub.register_full_backward_hook(self._make_bwd(layer)))
@@ -338,6 +417,7 @@ class GradSampleModule(nn.Module):
         for layer in self._layers:
             layer.passes_written = 0
             layer.pairs = []
+            layer.open_task = None
         self._multi_pending.clear()
         object.__setattr__(self, "_multi_task", None)
         if self._inflight:
@@ -367,6 +447,8 @@ class GradSampleModule(nn.Module):
     def _close(self):
         self.remove_hooks()
         for sub in self._module.modules():
+            if "_dpk_claim" in sub.__dict__:
+                object.__setattr__(sub, "_dpk_claim", None)
             if "_dpk_sink" in sub.__dict__:
                 object.__setattr__(sub, "_dpk_sink", None)
                 object.__setattr__(sub, "_dpk_sink_active", None)
@@ -412,12 +494,14 @@ class GradSampleModule(nn.Module):
                 if isinstance(output, torch.Tensor) and not output.requires_grad:
                     # first layer of the model (its input is data): nothing upstream needs a gradient, but the
                     # backward hook must still see grad_output -> keep the output in the graph at zero cost
-                    if self._tap.device != output.device:
-                        object.__setattr__(self, "_tap", torch.zeros((), device=output.device, requires_grad=True))
-                    tapped = _GradTap.apply(output, self._tap)
+                    tapped = _GradTap.apply(output, self._tap_on(output.device))
             if not self.hooks_enabled or not module.training or not torch.is_grad_enabled():
                 return tapped
-            layer.acts.append(inputs[0].detach())
+            if self.activation_bits == 8 and layer.kind == "linear":
+                kept = inputs[1] if len(inputs) > 1 else None
+                layer.acts.append(kept if isinstance(kept, Activation8) else compress_activation(inputs[0]))
+            else:
+                layer.acts.append(inputs[0].detach())
             layer.counter += 1
             for p in layer.params:
                 p._forward_counter += 1
@@ -433,6 +517,8 @@ class GradSampleModule(nn.Module):
             if g is None:
                 raise RuntimeError(f"{layer.name}: no gradient reached this layer's output")
             a = layer.acts.pop()  # LIFO: backward visits calls in reverse
+            if isinstance(a, Activation8):
+                a = restore_activation(a)
             layer.pairs.append((a, g.detach()))
             layer.counter -= 1
             for p in layer.params:
@@ -441,6 +527,11 @@ class GradSampleModule(nn.Module):
                 self._materialise(layer)
 
         return hook
+
+    def _tap_on(self, device):
+        if self._tap.device != device:
+            object.__setattr__(self, "_tap", torch.zeros((), device=device, requires_grad=True))
+        return self._tap
 
     # ---- the deferred contraction ---------------------------------------------------------------------
     def _stack(self, tensors: List[torch.Tensor], feat_dims: int, batch_first: Optional[bool] = None) -> torch.Tensor:
@@ -522,21 +613,7 @@ class GradSampleModule(nn.Module):
         if G.dtype != torch.float32 or (layer.kind != "embedding" and A.dtype != torch.float32):
             raise _native.DpkError(f"{layer.name}: only fp32 activations/backprops are supported")
         B = A.shape[0]
-        k = layer.passes_written  # index of the un-stepped backward pass this belongs to
-        if k >= 1 and self.forbid_grad_accumulation:
-            raise ValueError("Poisson sampling is not compatible with grad accumulation. You need to call "
-                             "optimizer.step() after every forward/backward pass or consider using "
-                             "BatchMemoryManager")
-        if k == len(arena.pass_B):
-            arena.pass_B.append(B)
-        elif k < len(arena.pass_B):
-            if arena.pass_B[k] != B:
-                raise ValueError(f"{layer.name}: batch size {B} differs from {arena.pass_B[k]} seen by other layers")
-        else:
-            raise RuntimeError("per-sample-gradient bookkeeping out of sync (missing zero_grad?)")
-        row0 = sum(arena.pass_B[:k])
-        arena.ensure(max(row0 + B, 1))
-        layer.passes_written += 1
+        k, row0 = self._claim_rows(layer, B)
         g_scale = float(B) if self.loss_reduction == "mean" else 1.0
         part = arena.part[row0:] if row0 else arena.part
         if B > 0 and self._side is not None:
@@ -563,6 +640,26 @@ class GradSampleModule(nn.Module):
         elif B > 0:
             self._launch(layer, m, A, G, arena, row0, part, g_scale)
         self._publish(m, arena, row0, B, k)
+
+    def _claim_rows(self, layer: _Layer, B: int):
+        """(index of the un-stepped backward pass a layer's gradients of B samples belong to, its first arena row)."""
+        arena = self.arena
+        k = layer.passes_written
+        if k >= 1 and self.forbid_grad_accumulation:
+            raise ValueError("Poisson sampling is not compatible with grad accumulation. You need to call "
+                             "optimizer.step() after every forward/backward pass or consider using "
+                             "BatchMemoryManager")
+        if k == len(arena.pass_B):
+            arena.pass_B.append(B)
+        elif k < len(arena.pass_B):
+            if arena.pass_B[k] != B:
+                raise ValueError(f"{layer.name}: batch size {B} differs from {arena.pass_B[k]} seen by other layers")
+        else:
+            raise RuntimeError("per-sample-gradient bookkeeping out of sync (missing zero_grad?)")
+        row0 = sum(arena.pass_B[:k])
+        arena.ensure(max(row0 + B, 1))
+        layer.passes_written += 1
+        return k, row0
 
     def _multi_eligible(self, layer, m, A, G, arena, B) -> bool:
         if layer.kind != "linear" or B > self.multi_launch_max_batch or self._side is not None:

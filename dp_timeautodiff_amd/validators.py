@@ -18,7 +18,8 @@ from typing import List
 import torch
 import torch.nn as nn
 
-from .layers import DPGRU, DPLSTM, DPMultiheadAttention, RNNLinear, SequenceBias
+from .layers import (DPCausalConv, DPGRU, DPLSTM, DPMultiheadAttention, DPRMSNorm, DPSelectiveScan, RNNLinear,
+                     SequenceBias)
 
 
 class UnsupportedModuleError(ValueError):
@@ -34,7 +35,8 @@ class ShouldReplaceModuleError(UnsupportedModuleError):
 
 
 # leaf types whose parameters are served by a HIP per-sample-gradient kernel
-SUPPORTED_PARAM_MODULES = (nn.Linear, RNNLinear, nn.Embedding, nn.LayerNorm, SequenceBias)
+SUPPORTED_PARAM_MODULES = (nn.Linear, RNNLinear, nn.Embedding, nn.LayerNorm, SequenceBias, DPRMSNorm, DPCausalConv,
+                           DPSelectiveScan)
 _BATCHNORM = (nn.BatchNorm1d, nn.BatchNorm2d, nn.BatchNorm3d, nn.SyncBatchNorm)
 _INSTANCENORM = (nn.InstanceNorm1d, nn.InstanceNorm2d, nn.InstanceNorm3d)
 
@@ -42,6 +44,17 @@ _INSTANCENORM = (nn.InstanceNorm1d, nn.InstanceNorm2d, nn.InstanceNorm3d)
 def clone_module(module: nn.Module) -> nn.Module:
     """Deep clone (parameters, buffers and submodule structure); the original is left untouched."""
     return copy.deepcopy(module)
+
+
+class _RMSNormOutput(DPRMSNorm):
+    """Stands where an nn.RMSNorm stood: called with one tensor, returns one."""
+
+    def forward(self, x):
+        return super().forward(x)[0]
+
+
+def _fixable_rms_norm(m: nn.Module) -> bool:
+    return type(m) is nn.RMSNorm and m.elementwise_affine and len(m.normalized_shape) == 1
 
 
 def _replace(root: nn.Module, name: str, new: nn.Module) -> nn.Module:
@@ -69,6 +82,9 @@ class ModuleValidator:
             elif isinstance(sub, nn.MultiheadAttention):
                 errors.append(ShouldReplaceModuleError(
                     f"{name or 'Main'}: nn.MultiheadAttention must be replaced by DPMultiheadAttention (fix())."))
+            elif _fixable_rms_norm(sub):
+                errors.append(ShouldReplaceModuleError(
+                    f"{name or 'Main'}: nn.RMSNorm must be replaced by DPRMSNorm (fix())."))
             elif isinstance(sub, _BATCHNORM):
                 errors.append(ShouldReplaceModuleError(
                     f"{name or 'Main'}: BatchNorm cannot support training with differential privacy. The reason "
@@ -84,7 +100,8 @@ class ModuleValidator:
                     errors.append(UnsupportedModuleError(
                         f"{name or 'Main'}: {type(sub).__name__} owns trainable parameters but has no "
                         "per-sample-gradient kernel in this build (supported: Linear, Embedding, LayerNorm, "
-                        "DPLSTM/DPGRU cells, DPMultiheadAttention, SequenceBias)."))
+                        "DPLSTM/DPGRU cells, DPMultiheadAttention, SequenceBias, DPRMSNorm, DPCausalConv, "
+                        "DPSelectiveScan)."))
         if strict and len(errors) > 0:
             raise UnsupportedModuleError(errors)
         return errors
@@ -98,7 +115,8 @@ class ModuleValidator:
         module = clone_module(module)
         # collect first, then replace (named_modules would otherwise walk into the new children)
         todo = [(n, m) for n, m in module.named_modules()
-                if isinstance(m, (nn.LSTM, nn.GRU, nn.MultiheadAttention) + _BATCHNORM + _INSTANCENORM)]
+                if isinstance(m, (nn.LSTM, nn.GRU, nn.MultiheadAttention) + _BATCHNORM + _INSTANCENORM)
+                or _fixable_rms_norm(m)]
         for name, sub in todo:
             new = cls._fixed(sub, **kwargs)
             if new is not sub:
@@ -128,6 +146,10 @@ class ModuleValidator:
                                        add_zero_attn=sub.add_zero_attn, kdim=sub.kdim, vdim=sub.vdim,
                                        batch_first=sub.batch_first)
             new.load_from_mha(sub)
+            return new
+        if _fixable_rms_norm(sub):
+            new = _RMSNormOutput(sub.normalized_shape[0], torch.finfo(sub.weight.dtype).eps if sub.eps is None else sub.eps)
+            new.load_state_dict(sub.state_dict())
             return new
         if isinstance(sub, _BATCHNORM):
             return nn.GroupNorm(min(32, sub.num_features), sub.num_features, affine=sub.affine)

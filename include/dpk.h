@@ -323,6 +323,99 @@ int dpk_lstm_backward(const float* const* dout, const float* const* dcT, const f
 int dpk_adam_step(const float* grad, float* exp_avg, float* exp_avg_sq, const int64_t* win_table,
                   const float* hyper, int n_windows, const float* step_dev, int64_t P, void* stream);
 
+/*
+ * K12..K15 — the state-space layer: RMS norm with the residual's addition, short causal convolution, selective scan, and
+ * activations held in 8 bits.  No counterpart in the reference, whose sequence layers are recurrences (K8, K10): these are the
+ * same step of a DP-SGD pass for a layer whose recurrence is elementwise.  Activations are fp32, bf16 or fp16 (`dtype`), read at
+ * element alignment through element strides (last dimension contiguous) and written contiguous; parameters, their gradients,
+ * states of the scan and all sums are fp32.  Every sum has a fixed order.
+ */
+#define DPK_F32 0
+#define DPK_BF16 1
+#define DPK_F16 2
+
+/*
+ * K12: r = X + RES (RES NULL: r = X and R is not needed), rstd = 1/sqrt(mean_c r^2 + eps), Y = r * rstd * W over rows of C <=
+ * 16384 elements.  R, rstd (rows floats) may be NULL.  Q [rows, C] and QE [rows, ceil(C/128)] (both or neither) receive Y in 8 bits, as
+ * dpk_compress_activation would hold it.
+ * backward: DX (nullable) = rstd * (g - xhat * mean_c(g * xhat)) + DR (nullable), g = DY * W, xhat = R * rstd.  The rows are `groups`
+ * groups of rows_per_group; DW (nullable) row (group * split + k) receives scale * sum of DY * xhat over the k-th of `split` parts of
+ * the group's rows (accumulate: is added to).  dpk_rms_norm_split says how many parts fill the chip; dpk_sum_rows joins them.
+ */
+int dpk_rms_norm_forward(const void* X, int64_t ld_x, const void* RES, int64_t ld_res, const float* W, void* Y, void* R,
+                         float* rstd, int8_t* Q, uint8_t* QE, int64_t rows, int C, float eps, int dtype, void* stream);
+int dpk_rms_norm_split(int64_t groups, int64_t rows_per_group);
+int dpk_rms_norm_backward(const void* R, int64_t ld_r, const void* DY, int64_t ld_dy, const void* DR, int64_t ld_dr,
+                          const float* W, const float* rstd, void* DX, float* DW, int64_t dw_stride, int64_t groups,
+                          int64_t rows_per_group, int split, int C, float scale, int accumulate, int dtype, void* stream);
+
+/*
+ * K13: p_t = bias + sum_i w[d,i] x_{t-W+1+i}, y = p or silu(p), W <= 4, w [D,W], bias [D] or NULL.  x [B,T,D] with strides; rows
+ * before 0 are `state` [B,W-1,D] (NULL: zeros).  lengths (nullable, device int [B]): rows at and behind lengths[b] are padding:
+ * y = 0 there.  state_out (nullable): the last W-1 rows of each sequence.
+ * backward: dx, dstate (nullable) from dy and dstate_out (nullable, gradient of state_out); dpar (nullable) row b * segments + s
+ * receives the weight gradients [D,W] of time segment s, scaled, and at dbias_off (< 0: none) those of the bias [D].
+ * `segments` is what dpk_causal_conv_segments says, or 1.  step: one token, x [B,D], state updated in place.
+ */
+int dpk_causal_conv_segments(int B, int T, int D);
+int dpk_causal_conv_forward(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, const void* state,
+                            const int* lengths, void* y, void* state_out, int B, int T, int D, int W, int silu, int dtype,
+                            void* stream);
+int dpk_causal_conv_backward(const void* x, int64_t x_sb, int64_t x_st, const void* dy, int64_t dy_sb, int64_t dy_st,
+                             const float* w, const float* bias, const void* state, const void* dstate_out, const int* lengths,
+                             void* dx, void* dstate, float* dpar, int64_t dpar_stride, int64_t dbias_off, int segments, int B,
+                             int T, int D, int W, int silu, float scale, int accumulate, int dtype, void* stream);
+int dpk_causal_conv_step(const void* x, int64_t x_sb, void* state, const float* w, const float* bias, void* y, int B, int D,
+                         int W, int silu, int dtype, void* stream);
+
+/*
+ * K14: dt = softplus(delta + dt_bias) (softplus = 0: the sum itself), A = -exp(A_log) [D,N], h_t = exp(dt A) h_{t-1} + dt Bm_t u_t,
+ * y = Cm_t . h_t + Dskip u_t, out = y silu(z).  u, delta, z [B,T,D], Bm, Cm [B,T,N], N <= DPK_SCAN_MAX_STATE; Dskip, z, dt_bias, h0
+ * [B,D,N], lengths [B] may be NULL.  Rows at and behind lengths[b] leave the state alone and give out = 0.
+ * kept: [B, ceil(T / dpk_selective_scan_group()), N, D] floats, written by forward where the backward pass is to follow (else NULL).
+ * nchunk, chunk: as dpk_selective_scan_chunks says (or 1 and T rounded up to the group); nchunk > 1 needs edge
+ * [nchunk, B, N, D] and span [nchunk, B, D] floats of scratch, not kept between the calls.
+ * backward: gradients of every input; dhT (nullable) is the gradient of the final state, dh0 (nullable) receives that of h0.
+ * dA (of A_log) [D,N], dD [D], dbias [D] (each nullable): row b * nchunk + c, par_stride floats apart, receives what chunk c of sequence b
+ * adds, scaled; with nchunk = 1 that is the per-sample gradient.  dbc: dpk_selective_scan_channel_blocks(D) * B * T * 2N floats where
+ * that count is above 1.   step: T = 1, state [B,D,N] updated in place.
+ */
+#define DPK_SCAN_MAX_STATE 32
+typedef struct {
+    const void *u, *delta, *Bm, *Cm, *z;
+    const float *A_log, *Dskip, *dt_bias, *h0;
+    const int* lengths;
+    float *kept, *edge, *span;
+    int64_t u_sb, u_st, delta_sb, delta_st, B_sb, B_st, C_sb, C_st, z_sb, z_st;
+    int B, T, D, N, softplus, nchunk, chunk, dtype;
+} dpk_scan_desc;
+typedef struct {
+    const void* dout;
+    const float* dhT;
+    void *du, *ddelta, *dB, *dC, *dz;
+    float *dh0, *dbc, *dA, *dD, *dbias;
+    int64_t dout_sb, dout_st, par_stride;
+    float scale;
+    int accumulate;
+} dpk_scan_grads;
+int dpk_selective_scan_chunks(int B, int T, int D, int* chunk);
+int dpk_selective_scan_group(void);
+int dpk_selective_scan_channel_blocks(int D);
+int dpk_selective_scan_forward(const dpk_scan_desc* s, void* out, float* hT, void* stream);
+int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_scan_grads* g, void* stream);
+int dpk_selective_scan_step(const dpk_scan_desc* s, float* state, void* out, void* stream);
+
+/*
+ * K15: X [rows, C] (row stride ld_x) as Q int8 [rows, C] and one exponent byte per block of 128 elements of a row, QE [rows,
+ * ceil(C/128)]: with k the least integer >= -126 such that max|x| <= 127 * 2^k, q = rint(x * 2^-k) and the byte is k + 127 (at k = 122 |q| is
+ * held to 63, so that no finite value restores as inf).  A block that holds an inf or NaN has the byte 255 and restores as NaN.  restore writes q * 2^k in any dtype.
+ * dpk_sum_rows: out[g][c] (+)= scale * sum_r in[g][r][c] in a fixed order (joins the partial parameter gradients of K12..K14).
+ */
+int dpk_compress_activation(const void* X, int64_t ld_x, int8_t* Q, uint8_t* QE, int64_t rows, int C, int dtype, void* stream);
+int dpk_restore_activation(const int8_t* Q, const uint8_t* QE, void* X, int64_t rows, int C, int dtype, void* stream);
+int dpk_sum_rows(const float* in, int groups, int rows, int64_t P, int64_t in_stride, float* out, int64_t out_stride,
+                 float scale, int accumulate, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
