@@ -70,9 +70,10 @@ EXPORTS = {
     "dpk_causal_conv_backward": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 8
                                  + [c_int64, c_int64] + [c_int] * 6 + [c_float, c_int, c_int, c_void_p]),
     "dpk_causal_conv_step": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
-    "dpk_selective_scan_chunks": (c_int, [c_int, c_int, c_int, c_void_p]),
+    "dpk_selective_scan_chunks": (c_int, [c_int, c_int, c_int, c_int, c_void_p]),
     "dpk_selective_scan_group": (c_int, []),
-    "dpk_selective_scan_channel_blocks": (c_int, [c_int]),
+    "dpk_selective_scan_state_rows": (c_int, [c_int]),
+    "dpk_selective_scan_channel_blocks": (c_int, [c_int, c_int]),
     "dpk_selective_scan_forward": (c_int, [c_void_p] * 4),
     "dpk_selective_scan_backward": (c_int, [c_void_p] * 3),
     "dpk_selective_scan_step": (c_int, [c_void_p] * 4),
@@ -944,13 +945,13 @@ class ScanInputs:
         self.lengths = _par(lengths, "lengths", (u.shape[0],), dev, torch.int32)
         self.softplus = bool(softplus)
 
-    def desc(self, kept=None):
+    def desc(self, kept=None, backward: bool = False):
         """dpk_scan_desc and the scratch it points at."""
         u = self.u
         b, t = (u.shape[0], u.shape[1]) if u.dim() == 3 else (u.shape[0], 1)
         d, n = self.A_log.shape
         chunk = c_int(0)
-        nchunk = load().dpk_selective_scan_chunks(b, t, d, ctypes.byref(chunk)) if u.dim() == 3 else 1
+        nchunk = load().dpk_selective_scan_chunks(b, t, d, int(backward), ctypes.byref(chunk)) if u.dim() == 3 else 1
         s = _ScanDesc()
         s.B, s.T, s.D, s.N, s.softplus, s.dtype = b, t, d, n, int(self.softplus), ACT_DTYPES[u.dtype]
         s.nchunk, s.chunk = nchunk, chunk.value if u.dim() == 3 else load().dpk_selective_scan_group()
@@ -978,7 +979,8 @@ def selective_scan_forward(inp: ScanInputs, want_kept: bool, want_state: bool):
     out = torch.empty(b, t, d, dtype=u.dtype, device=u.device)
     hT = torch.empty(b, d, n, dtype=torch.float32, device=u.device) if want_state else None
     g = lib.dpk_selective_scan_group()
-    kept = torch.empty(b, (t + g - 1) // g, n, d, dtype=torch.float32, device=u.device) if want_kept else None
+    kept = torch.empty(b, (t + g - 1) // g, lib.dpk_selective_scan_state_rows(n), d, dtype=torch.float32,
+                       device=u.device) if want_kept else None
     if b:
         with _on(u.device) as stream:
             s, scratch = inp.desc(kept)
@@ -1010,12 +1012,12 @@ def selective_scan_backward(inp: ScanInputs, kept, dout, dhT, want_dh0: bool, wa
     lib = load()
     if b:
         with _on(dev) as stream:
-            s, scratch = inp.desc(kept)
+            s, scratch = inp.desc(kept, True)
             g = _ScanGrads()
             g.dout, g.dout_sb, g.dout_st = dout.data_ptr(), dout.stride(0), dout.stride(1)
             for name, x in (("dhT", dhT), ("du", du), ("ddelta", ddelta), ("dB", dB), ("dC", dC), ("dz", dz), ("dh0", dh0)):
                 setattr(g, name, None if x is None else x.data_ptr())
-            blocks = lib.dpk_selective_scan_channel_blocks(d)
+            blocks = lib.dpk_selective_scan_channel_blocks(d, n)
             dbc = torch.empty(blocks, b, t, 2 * n, dtype=torch.float32, device=dev) if blocks > 1 else None
             g.dbc = None if dbc is None else dbc.data_ptr()
             direct = windows is not None and s.nchunk == 1

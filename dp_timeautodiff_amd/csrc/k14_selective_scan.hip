@@ -7,13 +7,16 @@
 //   ddt = q u + sum_n e_n A_n, dA_log_n = A_n sum_t e_n dt, dD = sum dy u, ddelta = ddt sigmoid(delta + dt_bias)
 // Rows at and behind lengths[b] have dt = 0: the state stays what it was, out and all gradients there are 0.
 //
-// A lane owns one channel and walks time with its N states in registers (rows of u, delta, z are contiguous over channels, so
-// every access of a wave is one run of memory); B_t and C_t are the same for all channels and are staged in LDS for GROUP
-// steps at a time.  Per state and step that is one v_exp_f32 (quarter rate) and four plain instructions forward, two and
-// about thirteen backward: at N = 16 the vector ALU and HBM are about equally loaded forward, and the ALU bounds backward.
+// Forward, a lane owns one channel and walks time with its N states in registers (rows of u, delta, z are contiguous over
+// channels, so every access of a wave is one run of memory); B_t and C_t are the same for all channels and are staged in LDS for
+// GROUP steps at a time.
 // The backward pass needs the states in reverse.  Undoing the recurrence would divide by decays near 0, so the forward pass
-// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16) and the backward pass
-// recomputes a group into registers.
+// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16), and the backward pass recomputes a
+// group's states and decays into registers.  So that three waves a SIMD fit (with eight states
+// a lane the group spilled, and waited for its spills: 3311 us against 1887 for the plainest form), a channel's states lie on LS = N / 4 lanes there; what
+// a channel has once per step (softplus, gates, loads, stores) is dealt over those lanes by step, passed round by lane swaps.
+// Per state and step: forward one v_exp_f32 (quarter rate) and four plain instructions, backward one and thirteen, and the sums
+// over channels for dB and dC, which take a halving tree over the lanes (about five more).
 // Sequences x channels / 64 is the number of waves; few long sequences are cut into chunks of time: each chunk's effect is
 // (decay, state from zero), which a short kernel joins in order, and the chunks then run side by side from their true states.
 #include "ssm_common.h"
@@ -27,7 +30,7 @@ struct ScanArgs {
     const float *A_log, *Dskip, *dt_bias, *h0, *dhT;
     const int* lengths;
     void *out, *du, *ddelta, *dB, *dC, *dz;
-    float *hT, *dh0, *kept;     // kept: [b][group][n][d]
+    float *hT, *dh0, *kept;     // kept: [b][group][n][d], n padded to 4, 8, 16 or 32
     float *edge, *span;         // chunk edges: [chunk][b][n][d] and sums of dt [chunk][b][d]
     float *dbc;                 // [d block][b][t][2N] partial sums of dB | dC, where a row of channels needs several workgroups
     float *dA, *dD, *dbias;     // parameter gradients, row (b * nchunk + chunk) of par_stride floats
@@ -70,16 +73,57 @@ __device__ __forceinline__ void stage_bc(const ScanArgs& a, int b, int t0, int e
     }
 }
 
+// The same in two halves: fetched into registers, put into LDS once the group before is done with its half of the buffer.
+template <int NT>
+struct Staged {
+    static constexpr int K = GROUP * 2 * NT / 64;   // a workgroup of one wave takes all K turns
+    float v[K];
+};
+template <typename T, int NT>
+__device__ __forceinline__ void fetch_bc(const ScanArgs& a, int b, int t0, int end, Staged<NT>& r) {
+#pragma unroll
+    for (int k = 0; k < Staged<NT>::K; ++k) {
+        const int i = threadIdx.x + k * blockDim.x;
+        const int q = i / (2 * NT), c = i % (2 * NT), n = c % NT;
+        r.v[k] = 0.f;
+        if (i < GROUP * 2 * NT && t0 + q < end && n < a.N)
+            r.v[k] = c < NT ? to_f32(((const T*)a.B)[(int64_t)b * a.B_sb + (int64_t)(t0 + q) * a.B_st + n])
+                            : to_f32(((const T*)a.C)[(int64_t)b * a.C_sb + (int64_t)(t0 + q) * a.C_st + n]);
+    }
+}
+template <int NT>
+__device__ __forceinline__ void put_bc(const Staged<NT>& r, float (&s)[GROUP][2 * NT]) {
+#pragma unroll
+    for (int k = 0; k < Staged<NT>::K; ++k) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i < GROUP * 2 * NT) (&s[0][0])[i] = r.v[k];
+    }
+}
+
+// Operands are read relative to their group's first row: a 64-bit address that the wave shares and a 32-bit byte offset a lane.
+template <typename T>
+__device__ __forceinline__ const char* group_row(const void* p, int64_t sb, int64_t st, int b, int t0) {
+    return (const char*)p + (b * sb + t0 * st) * (int64_t)sizeof(T);
+}
+template <typename T>
+__device__ __forceinline__ float at(const char* row, uint32_t bytes) {
+    return to_f32(*reinterpret_cast<const T*>(row + bytes));
+}
+template <typename T>
+__device__ __forceinline__ void put(char* row, uint32_t bytes, float v) {
+    *reinterpret_cast<T*>(row + bytes) = (T)v;
+}
+
 template <typename T>
 __device__ __forceinline__ float elem(const void* p, int64_t sb, int64_t st, int b, int t, int d) {
     return to_f32(((const T*)p)[(int64_t)b * sb + (int64_t)t * st + d]);
 }
 
-__device__ __forceinline__ float step_size(const ScanArgs& a, float pre) { return a.softplus ? softplus_f(pre) : pre; }
+__device__ __forceinline__ float step_size(const ScanArgs& a, float pre) { return a.softplus ? softplus_f(pre).value : pre; }
 
 // EDGE: only the chunk's state from zero and its sum of dt, for the chunks' joining
 template <typename T, int NT, bool EDGE>
-__global__ void __launch_bounds__(256) scan_forward_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_forward_kernel(ScanArgs a) {
     __shared__ float bc[2][GROUP][2 * NT];
     const Place p(a);
     const int end = seq_end(a, p.b);
@@ -100,28 +144,35 @@ __global__ void __launch_bounds__(256) scan_forward_kernel(ScanArgs a) {
     const float skip = a.Dskip ? a.Dskip[dd] : 0.f;
     float span = 0.f;
     const int ngroup = (a.T + GROUP - 1) / GROUP;
+    const uint32_t lane_in = (uint32_t)dd * sizeof(T), lane_out = (uint32_t)p.d * sizeof(T);
     int ph = 0;
     for (int t0 = p.t0; t0 < p.t1; t0 += GROUP, ph ^= 1) {
         if (!EDGE && a.kept && p.live) {
-            float* k = a.kept + (((int64_t)p.b * ngroup + t0 / GROUP) * a.N) * a.D + p.d;
+            char* k = (char*)(a.kept + ((int64_t)p.b * ngroup + t0 / GROUP) * NT * a.D);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                if (n < a.N) k[(int64_t)n * a.D] = h[n];
+                if (n < a.N) put<float>(k + (int64_t)n * a.D * 4, (uint32_t)p.d * 4u, h[n]);
         }
+        char* out = (char*)a.out + ((int64_t)p.b * a.T + t0) * a.D * (int64_t)sizeof(T);
         if (t0 < end) {
             float u[GROUP], dt[GROUP], z[GROUP];
+            const char* gu = group_row<T>(a.u, a.u_sb, a.u_st, p.b, t0);
+            const char* gd = group_row<T>(a.delta, a.delta_sb, a.delta_st, p.b, t0);
+            const char* gz = group_row<T>(a.z, a.z_sb, a.z_st, p.b, t0);
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
-                const int t = t0 + q < end ? t0 + q : end - 1;
-                u[q] = t0 + q < end ? elem<T>(a.u, a.u_sb, a.u_st, p.b, t, dd) : 0.f;
-                dt[q] = elem<T>(a.delta, a.delta_sb, a.delta_st, p.b, t, dd);
-                if (!EDGE && a.z) z[q] = elem<T>(a.z, a.z_sb, a.z_st, p.b, t, dd);
+                const uint32_t r = t0 + q < end ? q * (uint32_t)sizeof(T) : 0u;   // rows behind the sequence: the group's first
+                u[q] = at<T>(gu, lane_in + r * (uint32_t)a.u_st);
+                dt[q] = at<T>(gd, lane_in + r * (uint32_t)a.delta_st);
+                if (!EDGE && a.z) z[q] = at<T>(gz, lane_in + r * (uint32_t)a.z_st);
             }
             stage_bc<T, NT>(a, p.b, t0, end, bc[ph]);
             __syncthreads();
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
-                dt[q] = t0 + q < end ? step_size(a, dt[q] + bias) : 0.f;
+                const bool in = t0 + q < end;
+                u[q] = in ? u[q] : 0.f;
+                dt[q] = in ? step_size(a, dt[q] + bias) : 0.f;
                 if (EDGE) span += dt[q];
             }
 #pragma unroll
@@ -135,14 +186,13 @@ __global__ void __launch_bounds__(256) scan_forward_kernel(ScanArgs a) {
                 }
                 if (!EDGE) {
                     if (a.z) y *= z[q] * sigmoid_f(z[q]);
-                    if (p.live && t0 + q < p.t1)
-                        ((T*)a.out)[((int64_t)p.b * a.T + t0 + q) * a.D + p.d] = (T)(t0 + q < end ? y : 0.f);
+                    if (p.live && t0 + q < p.t1) put<T>(out + (int64_t)q * a.D * (int64_t)sizeof(T), lane_out, t0 + q < end ? y : 0.f);
                 }
             }
         } else if (!EDGE && p.live) {
 #pragma unroll
             for (int q = 0; q < GROUP; ++q)
-                if (t0 + q < p.t1) ((T*)a.out)[((int64_t)p.b * a.T + t0 + q) * a.D + p.d] = (T)0.f;
+                if (t0 + q < p.t1) put<T>(out + (int64_t)q * a.D * (int64_t)sizeof(T), lane_out, 0.f);
         }
     }
     if (!p.live) return;
@@ -159,29 +209,67 @@ __global__ void __launch_bounds__(256) scan_forward_kernel(ScanArgs a) {
 }
 
 // Joins the chunks: edge[c] comes in as what chunk c makes of a zero start and goes out as its true start (forward) or the
-// gradient that enters it from behind (reverse).
+// gradient that enters it from behind (reverse).  Eight lanes share a state: each takes a run of eight chunks into registers, the
+// runs' (decay, state from zero) are joined by lane shuffles, and each lane walks its run again from its true start.
 template <bool REVERSE>
 __global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    constexpr int RUN = 8, LANES = 8;
     const int64_t per = (int64_t)a.N * a.D;
-    if (i >= a.nb * per) return;
-    const int b = (int)(i / per);
-    const int n = (int)(i % per / a.D), d = (int)(i % a.D);
+    // 8 neighbouring states and 8 runs a wave: lane = run * 8 + state
+    const int run = (threadIdx.x & 63) >> 3;
+    const int64_t i = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 8 + (threadIdx.x & 7);
+    const bool live = i < a.nb * per;
+    const int64_t at = live ? i : 0;
+    const int b = (int)(at / per);
+    const int n = (int)(at % per / a.D), d = (int)(at % a.D);
     const float A2 = -expf(a.A_log[(int64_t)d * a.N + n]) * LOG2E;
     const float* first = REVERSE ? a.dhT : a.h0;
     float h = first ? first[((int64_t)b * a.D + d) * a.N + n] : 0.f;
-    for (int k = 0; k < a.nchunk; ++k) {
-        const int c = REVERSE ? a.nchunk - 1 - k : k;
-        float* e = a.edge + (((int64_t)c * a.nb + b) * a.N + n) * a.D + d;
-        const float own = *e;
-        *e = h;
-        h = own + exp2_hw(A2 * a.span[((int64_t)c * a.nb + b) * a.D + d]) * h;
+    for (int k0 = 0; k0 < a.nchunk; k0 += RUN * LANES) {
+        float own[RUN], decay[RUN];
+        float f = 1.f, z = 0.f;   // the run as h -> f h + z
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) {
+            const int c = k0 + run * RUN + k;
+            const bool in = c < a.nchunk;
+            const int64_t cb = (int64_t)(REVERSE ? a.nchunk - 1 - (in ? c : 0) : (in ? c : 0)) * a.nb + b;
+            const float o = a.edge[(cb * a.N + n) * a.D + d], s = a.span[cb * a.D + d];
+            own[k] = in ? o : 0.f;
+            decay[k] = in ? s : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) {
+            decay[k] = exp2_hw(A2 * decay[k]);
+            z = own[k] + decay[k] * z;
+            f *= decay[k];
+        }
+#pragma unroll
+        for (int off = 1; off < LANES; off <<= 1) {   // joined with all runs before it
+            const float pf = __shfl_up(f, 8 * off, 64), pz = __shfl_up(z, 8 * off, 64);
+            if (run >= off) {
+                z = z + f * pz;
+                f *= pf;
+            }
+        }
+        const float pf = __shfl_up(f, 8, 64), pz = __shfl_up(z, 8, 64);
+        float g = run ? pz + pf * h : h;
+        const float lf = __shfl(f, 56 + (threadIdx.x & 7), 64), lz = __shfl(z, 56 + (threadIdx.x & 7), 64);
+        h = lz + lf * h;
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) {
+            const int c = k0 + run * RUN + k;
+            if (c < a.nchunk && live) {
+                const int64_t cb = (int64_t)(REVERSE ? a.nchunk - 1 - c : c) * a.nb + b;
+                a.edge[(cb * a.N + n) * a.D + d] = g;
+            }
+            g = own[k] + decay[k] * g;
+        }
     }
 }
 
 // what a chunk hands to the chunk before it if nothing enters it from behind
 template <typename T, int NT>
-__global__ void __launch_bounds__(256) scan_backward_edge_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_backward_edge_kernel(ScanArgs a) {
     __shared__ float bc[2][GROUP][2 * NT];
     const Place p(a);
     const int end = seq_end(a, p.b);
@@ -193,31 +281,35 @@ __global__ void __launch_bounds__(256) scan_backward_edge_kernel(ScanArgs a) {
         dh[n] = 0.f;
     }
     const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f;
+    const uint32_t lane_in = (uint32_t)dd * sizeof(T);
     float span = 0.f;
     int ph = 0;
-    const int last = p.t0 + (p.t1 - p.t0 - 1) / GROUP * GROUP;
-    for (int t0 = last; t0 >= p.t0; t0 -= GROUP, ph ^= 1) {
+    for (int t0 = p.t0 + (p.t1 - p.t0 - 1) / GROUP * GROUP; t0 >= p.t0; t0 -= GROUP) {
         if (t0 >= end) continue;
-        float dy[GROUP], dt[GROUP];
+        float dy[GROUP], dt[GROUP], z[GROUP];
+        const char* gd = group_row<T>(a.delta, a.delta_sb, a.delta_st, p.b, t0);
+        const char* go = group_row<T>(a.dout, a.dout_sb, a.dout_st, p.b, t0);
+        const char* gz = group_row<T>(a.z, a.z_sb, a.z_st, p.b, t0);
 #pragma unroll
         for (int q = 0; q < GROUP; ++q) {
-            const int t = t0 + q < end ? t0 + q : end - 1;
-            dt[q] = elem<T>(a.delta, a.delta_sb, a.delta_st, p.b, t, dd);
-            dy[q] = elem<T>(a.dout, a.dout_sb, a.dout_st, p.b, t, dd);
-            if (a.z) {
-                const float z = elem<T>(a.z, a.z_sb, a.z_st, p.b, t, dd);
-                dy[q] *= z * sigmoid_f(z);
-            }
+            const uint32_t r = t0 + q < end ? q * (uint32_t)sizeof(T) : 0u;
+            dt[q] = at<T>(gd, lane_in + r * (uint32_t)a.delta_st);
+            dy[q] = at<T>(go, lane_in + r * (uint32_t)a.dout_st);
+            z[q] = at<T>(gz, lane_in + r * (uint32_t)a.z_st);
         }
         stage_bc<T, NT>(a, p.b, t0, end, bc[ph]);
         __syncthreads();
 #pragma unroll
         for (int q = GROUP - 1; q >= 0; --q) {
-            const float s = t0 + q < end ? step_size(a, dt[q] + bias) : 0.f;
+            __builtin_amdgcn_sched_barrier(0);
+            const bool in = t0 + q < end;
+            const float s = in ? step_size(a, dt[q] + bias) : 0.f;
+            const float g = in ? (a.dz ? dy[q] * (z[q] * sigmoid_f(z[q])) : dy[q]) : 0.f;
             span += s;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) dh[n] = exp2_hw(s * A2[n]) * (dh[n] + dy[q] * bc[ph][q][NT + n]);
+            for (int n = 0; n < NT; ++n) dh[n] = exp2_hw(s * A2[n]) * (dh[n] + g * bc[ph][q][NT + n]);
         }
+        ph ^= 1;
     }
     if (!p.live) return;
 #pragma unroll
@@ -226,8 +318,8 @@ __global__ void __launch_bounds__(256) scan_backward_edge_kernel(ScanArgs a) {
     a.span[((int64_t)p.chunk * a.nb + p.b) * a.D + p.d] = span;
 }
 
-// Sums each of V values over the 64 lanes of a wave; afterwards lane l holds the sum of value slot(l).  A step adds the halves
-// of two values at once and leaves one register of the two, so V values take about 2 V instructions instead of 6 V.
+// Sums each of V values over lanes; afterwards lane l holds the sum of value lane_slot(l).  A step adds the halves of two values
+// at once and leaves one register of the two, so V values take about 2 V instructions instead of one per value and lane bit.
 template <int C>
 __device__ __forceinline__ void fold32(float* v) {
 #pragma unroll
@@ -259,162 +351,273 @@ __device__ __forceinline__ void fold_dpp(float* v) {
     }
 }
 constexpr int half_of(int c) { return c > 1 ? c / 2 : 1; }
-template <int V>   // V a power of two, 8..64
-__device__ __forceinline__ void lane_sums(float* v) {
-    constexpr int C3 = V / 4, C4 = half_of(C3), C5 = half_of(C4), C6 = half_of(C5);
-    fold32<V>(v);
-    fold16<V / 2>(v);
-    fold_dpp<C3, 0x128, 8>(v);    // row_ror:8
-    fold_dpp<C4, 0x141, 4>(v);    // row_half_mirror
-    fold_dpp<C5, 0x4E, 2>(v);     // quad_perm 2,3,0,1
-    fold_dpp<C6, 0xB1, 1>(v);     // quad_perm 1,0,3,2
+// V = 4 values over the 64 / LS low lanes
+template <int LS>
+__device__ __forceinline__ float lane_sums(float (&v)[4]) {
+    constexpr int C1 = LS == 1 ? 2 : 4, C2 = LS <= 2 ? half_of(C1) : 4, C3 = LS <= 4 ? half_of(C2) : 4;
+    constexpr int C4 = half_of(C3), C5 = half_of(C4);
+    if constexpr (LS == 1) fold32<4>(v);
+    if constexpr (LS <= 2) fold16<C1>(v);
+    if constexpr (LS <= 4) fold_dpp<C2, 0x128, 8>(v);   // row_ror:8
+    fold_dpp<C3, 0x141, 4>(v);                          // row_half_mirror
+    fold_dpp<C4, 0x4E, 2>(v);                           // quad_perm 2,3,0,1
+    fold_dpp<C5, 0xB1, 1>(v);                           // quad_perm 1,0,3,2
+    return v[0];
 }
-template <int V>
-__device__ __forceinline__ int lane_slot(int lane) {
-    int s = 0, c = V;
+template <int LS>
+__device__ __forceinline__ int lane_slot(int lane) {   // which of the four values the lane ends up with
+    int s = 0, c = 4;
 #pragma unroll
-    for (int bit = 32; bit >= 1; bit >>= 1) {
+    for (int bit = 32 / LS; bit >= 1; bit >>= 1) {
         c >>= 1;
         if (c >= 1 && (lane & bit)) s += c;
     }
     return s;
 }
-// one lane of each set that holds the same sum
-template <int V>
-__device__ __forceinline__ bool lane_writes(int lane) {
-    return (lane & (64 / (V < 64 ? V : 64) - 1)) == 0;
+
+// Lane part s = lane / (64 / LS) of a channel owns the steps s * GROUP / LS ...; all[q] becomes every lane's copy of step q.
+template <int LS>
+__device__ __forceinline__ void spread(const float (&own)[GROUP / LS], float (&all)[GROUP]) {
+    constexpr int OWN = GROUP / LS;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+        float v8[LS == 8 ? 2 : 1];
+        if constexpr (LS == 8) {
+            const float other = dpp<0x128>(own[i]);
+            const bool up = threadIdx.x & 8;
+            v8[0] = up ? other : own[i];
+            v8[1] = up ? own[i] : other;
+        } else {
+            v8[0] = own[i];
+        }
+        constexpr int N8 = LS == 8 ? 2 : 1, N16 = LS >= 4 ? 2 : 1, N32 = LS >= 2 ? 2 : 1;
+#pragma unroll
+        for (int k8 = 0; k8 < N8; ++k8) {
+            float v16[2] = {v8[k8], 0.f};
+            if constexpr (LS >= 4) {
+                const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v8[k8]), __float_as_uint(v8[k8]), false, false);
+                v16[0] = __uint_as_float(r[0]);
+                v16[1] = __uint_as_float(r[1]);
+            }
+#pragma unroll
+            for (int k16 = 0; k16 < N16; ++k16) {
+                float v32[2] = {v16[k16], 0.f};
+                if constexpr (LS >= 2) {
+                    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v16[k16]), __float_as_uint(v16[k16]), false, false);
+                    v32[0] = __uint_as_float(r[0]);
+                    v32[1] = __uint_as_float(r[1]);
+                }
+#pragma unroll
+                for (int k32 = 0; k32 < N32; ++k32) all[((k32 * N16 + k16) * N8 + k8) * OWN + i] = v32[k32];
+            }
+        }
+    }
+}
+// The sums over a channel's lanes, each step's at its owner; leaves them in all[0 .. GROUP / LS).
+template <int LS>
+__device__ __forceinline__ void collect(float (&all)[GROUP]) {
+    if constexpr (LS >= 2) fold32<GROUP>(all);
+    if constexpr (LS >= 4) fold16<GROUP / 2>(all);
+    if constexpr (LS >= 8) fold_dpp<GROUP / 4, 0x128, 8>(all);
 }
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(256) scan_backward_kernel(ScanArgs a) {
+template <typename T, int LS>
+__global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
+    constexpr int S = 4, NT = S * LS, CPW = 64 / LS, OWN = GROUP / LS;
     __shared__ float bc[2][GROUP][2 * NT];
     __shared__ float part[2][4][GROUP][2 * NT];
-    const Place p(a);
-    const int end = seq_end(a, p.b);
-    const int dd = p.live ? p.d : a.D - 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    float A2[NT], dh[NT], dA[NT];
+    const int sb = lane / CPW, n0 = sb * S, q0 = sb * OWN;
+    const int part_slot = lane_slot<LS>(lane) + n0;
+    const int dblk = blockIdx.x % a.ndb, rest = blockIdx.x / a.ndb;
+    const int b = rest % a.nb, chunk = rest / a.nb;
+    const int d = (dblk * nw + wave) * CPW + lane % CPW;
+    const bool live = d < a.D;
+    const int dd = live ? d : a.D - 1;
+    const int lo = chunk * a.chunk, hi = lo + a.chunk < a.T ? lo + a.chunk : a.T;
+    const int end = seq_end(a, b);
+    float A2[S], dh[S], dA[S];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        A2[n] = n < a.N ? -expf(a.A_log[(int64_t)dd * a.N + n]) * LOG2E : 0.f;
-        dA[n] = 0.f;
-        dh[n] = 0.f;
-        if (n < a.N) {
+    for (int j = 0; j < S; ++j) {
+        const int n = n0 + j;
+        A2[j] = n < a.N ? -expf(a.A_log[(int64_t)dd * a.N + n]) * LOG2E : 0.f;
+        dA[j] = 0.f;
+        dh[j] = 0.f;
+        if (n < a.N && live) {   // lanes behind the last channel stay 0: nothing of them may reach the sums over channels
             if (a.nchunk > 1)
-                dh[n] = a.edge[(((int64_t)p.chunk * a.nb + p.b) * a.N + n) * a.D + dd];
+                dh[j] = a.edge[(((int64_t)chunk * a.nb + b) * a.N + n) * a.D + dd];
             else if (a.dhT)
-                dh[n] = a.dhT[((int64_t)p.b * a.D + dd) * a.N + n];
+                dh[j] = a.dhT[((int64_t)b * a.D + dd) * a.N + n];
         }
-        if (!p.live) dh[n] = 0.f;   // nothing of these lanes may reach the sums over channels
     }
     const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f;
     const float skip = a.Dskip ? a.Dskip[dd] : 0.f;
     float dD = 0.f, dbias = 0.f;
     const int ngroup = (a.T + GROUP - 1) / GROUP;
+    // The group being fetched, as it lies in memory.  Steps behind the sequence read the group's first row instead and count as
+    // zeros where the group is taken up, as do lanes behind the last channel.  (Not here: a choice right behind a load becomes a
+    // branch round it and a wait for it, in the middle of the arithmetic that is to hide it.)
+    float nu[OWN], npre[OWN], ndy[OWN], nz[OWN], nh[S];
+    Staged<NT> nbc;
+    const uint32_t first = (uint32_t)dd * sizeof(T);
+    const uint32_t lane_u = (uint32_t)(q0 * a.u_st + dd) * sizeof(T), lane_pre = (uint32_t)(q0 * a.delta_st + dd) * sizeof(T);
+    const uint32_t lane_dy = (uint32_t)(q0 * a.dout_st + dd) * sizeof(T), lane_z = (uint32_t)(q0 * a.z_st + dd) * sizeof(T);
+    const uint32_t lane_out = ((uint32_t)q0 * a.D + d) * sizeof(T);
+    const bool gate = a.dz != nullptr;   // without a gate a.z is a.u: read, and not used
+    const uint32_t lane_kept = ((uint32_t)n0 * a.D + dd) * 4u;
+    auto fetch = [&](int t0) {
+        const char* gu = group_row<T>(a.u, a.u_sb, a.u_st, b, t0);
+        const char* gd = group_row<T>(a.delta, a.delta_sb, a.delta_st, b, t0);
+        const char* go = group_row<T>(a.dout, a.dout_sb, a.dout_st, b, t0);
+        const char* gz = group_row<T>(a.z, a.z_sb, a.z_st, b, t0);
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            const bool in = t0 + q0 + i < end;
+            const uint32_t es = (uint32_t)i * sizeof(T);
+            nu[i] = at<T>(gu, in ? lane_u + es * (uint32_t)a.u_st : first);
+            npre[i] = at<T>(gd, in ? lane_pre + es * (uint32_t)a.delta_st : first);
+            ndy[i] = at<T>(go, in ? lane_dy + es * (uint32_t)a.dout_st : first);
+            nz[i] = at<T>(gz, in ? lane_z + es * (uint32_t)a.z_st : first);
+        }
+        const char* k = (const char*)(a.kept + ((int64_t)b * ngroup + t0 / GROUP) * NT * a.D);
+#pragma unroll
+        for (int j = 0; j < S; ++j) nh[j] = at<float>(k, lane_kept + (uint32_t)j * (uint32_t)a.D * 4u);
+    };
+    int t0 = lo + (hi - lo - 1) / GROUP * GROUP;
+    for (; t0 >= lo && t0 >= end; t0 -= GROUP) {   // groups behind the sequence
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            if (live && t0 + q0 + i < hi) {
+                const int64_t o = ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T);
+                put<T>((char*)a.du + o, lane_out, 0.f);
+                put<T>((char*)a.ddelta + o, lane_out, 0.f);
+                if (a.dz) put<T>((char*)a.dz + o, lane_out, 0.f);
+            }
+        }
+        for (int i = threadIdx.x; i < GROUP * 2 * a.N; i += blockDim.x) {
+            const int q = i / (2 * a.N), r = i % (2 * a.N);
+            if (t0 + q >= hi) continue;
+            const int64_t row = (int64_t)b * a.T + t0 + q;
+            if (a.ndb > 1)
+                a.dbc[((int64_t)dblk * a.nb * a.T + row) * 2 * a.N + r] = 0.f;
+            else if (r < a.N)
+                ((T*)a.dB)[row * a.N + r] = (T)0.f;
+            else
+                ((T*)a.dC)[row * a.N + r - a.N] = (T)0.f;
+        }
+    }
     int ph = 0;
-    const int last = p.t0 + (p.t1 - p.t0 - 1) / GROUP * GROUP;
-    for (int t0 = last; t0 >= p.t0; t0 -= GROUP) {
-        if (t0 >= end) {
+    if (t0 >= lo) {
+        fetch(t0);
+        fetch_bc<T, NT>(a, b, t0, end, nbc);
+        put_bc<NT>(nbc, bc[0]);
+        __syncthreads();
+    }
+    for (; t0 >= lo; t0 -= GROUP) {
+        float u[OWN], slope[OWN], gs[OWN], dts[OWN], zf[OWN];
+        float dt[GROUP], x[GROUP], g[GROUP], into[GROUP], along[GROUP], y[GROUP];
+        float e[GROUP][S], eh[GROUP][S];   // decay, and what it leaves of the state before the step
+        const int next = t0 - GROUP >= lo ? t0 - GROUP : t0;   // (the first group is fetched twice)
+        fetch_bc<T, NT>(a, b, next, end, nbc);
+        {
+            float xs[OWN];
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                const bool in = t0 + q0 + i < end && live;
+                const float z = in ? nz[i] : 0.f, dy = in ? ndy[i] : 0.f, sg = sigmoid_f(z);
+                const float pre = npre[i] + bias;
+                const Softplus s = softplus_f(in ? pre : 0.f);
+                u[i] = in ? nu[i] : 0.f;
+                dts[i] = in ? (a.softplus ? s.value : pre) : 0.f;
+                slope[i] = a.softplus ? s.slope : 1.f;
+                gs[i] = gate ? dy * z * sg : dy;
+                zf[i] = dy * sg * (1.f + z * (1.f - sg));
+                xs[i] = dts[i] * u[i];
+                dD += gs[i] * u[i];
+            }
+            spread<LS>(dts, dt);
+            spread<LS>(xs, x);
+            spread<LS>(gs, g);
+        }
+        // Steps are kept apart for the scheduler, which would otherwise fetch all of a group's B and C at once.
+        {
+            float h[S];
+#pragma unroll
+            for (int j = 0; j < S; ++j) h[j] = n0 + j < a.N && live ? nh[j] : 0.f;
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
-                if (t0 + q >= p.t1) break;
-                if (p.live) {
-                    const int64_t o = ((int64_t)p.b * a.T + t0 + q) * a.D + p.d;
-                    ((T*)a.du)[o] = (T)0.f;
-                    ((T*)a.ddelta)[o] = (T)0.f;
-                    if (a.dz) ((T*)a.dz)[o] = (T)0.f;
+                float v[S];
+                y[q] = 0.f;
+#pragma unroll
+                for (int j = 0; j < S; ++j) {
+                    e[q][j] = exp2_hw(dt[q] * A2[j]);
+                    eh[q][j] = e[q][j] * h[j];
+                    h[j] = eh[q][j] + x[q] * bc[ph][q][n0 + j];
+                    y[q] += bc[ph][q][NT + n0 + j] * h[j];
+                    v[j] = g[q] * h[j];
                 }
-                for (int i = threadIdx.x; i < 2 * a.N; i += blockDim.x) {
-                    const int64_t row = (int64_t)p.b * a.T + t0 + q;
-                    if (a.ndb > 1)
-                        a.dbc[((int64_t)p.dblk * a.nb * a.T + row) * 2 * a.N + i] = 0.f;
-                    else if (i < a.N)
-                        ((T*)a.dB)[row * a.N + i] = (T)0.f;
-                    else
-                        ((T*)a.dC)[row * a.N + i - a.N] = (T)0.f;
-                }
+                part[ph][wave][q][NT + part_slot] = lane_sums<LS>(v);   // lanes that hold the same sum write it to the same place
             }
-            continue;
         }
-        float u[GROUP], pre[GROUP], dy[GROUP], z[GROUP], dt[GROUP], hist[GROUP][NT];
+        collect<LS>(y);
+        if (gate) {
 #pragma unroll
-        for (int q = 0; q < GROUP; ++q) {
-            // steps behind the sequence and lanes behind the last channel count as zeros, whatever lies there: neither may
-            // bring an inf or NaN into the sums over channels
-            const bool in = t0 + q < end && p.live;
-            const int t = t0 + q < end ? t0 + q : end - 1;
-            u[q] = in ? elem<T>(a.u, a.u_sb, a.u_st, p.b, t, dd) : 0.f;
-            pre[q] = in ? elem<T>(a.delta, a.delta_sb, a.delta_st, p.b, t, dd) + bias : 0.f;
-            dy[q] = in ? elem<T>(a.dout, a.dout_sb, a.dout_st, p.b, t, dd) : 0.f;
-            z[q] = in && a.z ? elem<T>(a.z, a.z_sb, a.z_st, p.b, t, dd) : 0.f;
+            for (int i = 0; i < OWN; ++i) {
+                const int t = t0 + q0 + i;
+                if (live && t < hi)
+                    put<T>((char*)a.dz + ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T), lane_out, t < end ? zf[i] * (y[i] + skip * u[i]) : 0.f);
+            }
         }
-        {
-            const float* k = a.kept + (((int64_t)p.b * ngroup + t0 / GROUP) * a.N) * a.D + dd;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) hist[0][n] = n < a.N && p.live ? k[(int64_t)n * a.D] : 0.f;
-        }
-        stage_bc<T, NT>(a, p.b, t0, end, bc[ph]);
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < GROUP; ++q) dt[q] = t0 + q < end ? step_size(a, pre[q]) : 0.f;
-#pragma unroll
-        for (int q = 0; q + 1 < GROUP; ++q) {
-            const float x = dt[q] * u[q];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) hist[q + 1][n] = exp2_hw(dt[q] * A2[n]) * hist[q][n] + x * bc[ph][q][n];
-        }
+        asm volatile("" ::: "memory");   // B and C are read from LDS again rather than held for all steps
 #pragma unroll
         for (int q = GROUP - 1; q >= 0; --q) {
-            const float x = dt[q] * u[q];
-            float g = dy[q], sg = 1.f;
-            if (a.z) {
-                sg = sigmoid_f(z[q]);
-                g *= z[q] * sg;
-            }
-            float y = skip * u[q], into = 0.f, along = 0.f;
-            float v[2 * NT];
+            // half of the group's registers are free again: the next group's operands come in behind the other half
+            if (q == GROUP / 2 - 1) fetch(next);
+            float v[S];
+            into[q] = along[q] = 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float e = exp2_hw(dt[q] * A2[n]);
-                const float eh = e * hist[q][n];
-                const float h = eh + x * bc[ph][q][n];
-                const float cn = bc[ph][q][NT + n];
-                y += cn * h;
-                dh[n] += g * cn;
-                v[n] = dh[n] * x;
-                v[NT + n] = g * h;
-                into += dh[n] * bc[ph][q][n];
-                const float t = dh[n] * eh;
-                along += t * A2[n];
-                dA[n] += t * dt[q];
-                dh[n] *= e;
+            for (int j = 0; j < S; ++j) {
+                dh[j] += g[q] * bc[ph][q][NT + n0 + j];
+                v[j] = dh[j] * x[q];
+                into[q] += dh[j] * bc[ph][q][n0 + j];
+                const float t = dh[j] * eh[q][j];
+                along[q] += t * A2[j];
+                dA[j] += t * dt[q];
+                dh[j] *= e[q][j];
+                asm volatile("" : "+v"(dA[j]));   // summed here, not behind the group with eight steps' t held until then
             }
-            lane_sums<2 * NT>(v);
-            if (lane_writes<2 * NT>(lane)) part[ph][wave][q][lane_slot<2 * NT>(lane)] = v[0];
-            const bool in = t0 + q < end;
-            const float ddt = into * u[q] + along * LN2;
-            const float dpre = a.softplus ? ddt * sigmoid_f(pre[q]) : ddt;
-            if (in) {
-                dD += g * u[q];
-                dbias += dpre;
-            }
-            if (p.live && t0 + q < p.t1) {
-                const int64_t o = ((int64_t)p.b * a.T + t0 + q) * a.D + p.d;
-                ((T*)a.du)[o] = (T)(in ? into * dt[q] + skip * g : 0.f);
-                ((T*)a.ddelta)[o] = (T)(in ? dpre : 0.f);
-                if (a.dz) ((T*)a.dz)[o] = (T)(in ? dy[q] * y * sg * (1.f + z[q] * (1.f - sg)) : 0.f);
+            part[ph][wave][q][part_slot] = lane_sums<LS>(v);
+        }
+        // Wait for the next group's operands here, before this group's stores: a wait behind them would be one for them as well.
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) asm volatile("" : "+v"(nu[i]), "+v"(npre[i]), "+v"(ndy[i]), "+v"(nz[i]));
+#pragma unroll
+        for (int j = 0; j < S; ++j) asm volatile("" : "+v"(nh[j]));
+        put_bc<NT>(nbc, bc[ph ^ 1]);
+        collect<LS>(into);
+        collect<LS>(along);
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            const int t = t0 + q0 + i;
+            const bool in = t < end;
+            const float dpre = (into[i] * u[i] + along[i] * LN2) * slope[i];
+            if (in) dbias += dpre;
+            if (live && t < hi) {
+                const int64_t o = ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T);
+                put<T>((char*)a.du + o, lane_out, in ? into[i] * dts[i] + skip * gs[i] : 0.f);
+                put<T>((char*)a.ddelta + o, lane_out, in ? dpre : 0.f);
             }
         }
-        __syncthreads();
+        __syncthreads();   // the group's sums are written, the next group's B and C staged
         for (int i = threadIdx.x; i < GROUP * 2 * NT; i += blockDim.x) {
             const int q = i / (2 * NT), r = i % (2 * NT), n = r % NT;
-            if (n >= a.N || t0 + q >= p.t1) continue;
+            if (n >= a.N || t0 + q >= hi) continue;
             float s = 0.f;
             if (t0 + q < end)
                 for (int w = 0; w < nw; ++w) s += part[ph][w][q][r];
-            const int64_t row = (int64_t)p.b * a.T + t0 + q;
+            const int64_t row = (int64_t)b * a.T + t0 + q;
             if (a.ndb > 1)
-                a.dbc[((int64_t)p.dblk * a.nb * a.T + row) * 2 * a.N + (r < NT ? n : a.N + n)] = s;
+                a.dbc[((int64_t)dblk * a.nb * a.T + row) * 2 * a.N + (r < NT ? n : a.N + n)] = s;
             else if (r < NT)
                 ((T*)a.dB)[row * a.N + n] = (T)s;
             else
@@ -422,21 +625,28 @@ __global__ void __launch_bounds__(256) scan_backward_kernel(ScanArgs a) {
         }
         ph ^= 1;
     }
-    if (!p.live) return;
-    if (a.dh0 && p.chunk == 0) {
+    if (a.dh0 && chunk == 0 && live) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (n < a.N) a.dh0[((int64_t)p.b * a.D + p.d) * a.N + n] = dh[n];
+        for (int j = 0; j < S; ++j)
+            if (n0 + j < a.N) a.dh0[((int64_t)b * a.D + d) * a.N + n0 + j] = dh[j];
     }
-    const int64_t row = ((int64_t)p.b * a.nchunk + p.chunk) * a.par_stride;
+    // dD and dbias are spread over the channel's lanes by step
+#pragma unroll
+    for (int off = CPW; off < 64; off <<= 1) {
+        dD += __shfl_xor(dD, off, 64);
+        dbias += __shfl_xor(dbias, off, 64);
+    }
+    if (!live) return;
+    const int64_t row = ((int64_t)b * a.nchunk + chunk) * a.par_stride;
     if (a.dA) {
-        float* o = a.dA + row + (int64_t)p.d * a.N;
+        float* o = a.dA + row + (int64_t)d * a.N + n0;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (n < a.N) o[n] = (a.accumulate ? o[n] : 0.f) + a.scale * (A2[n] * LN2) * dA[n];
+        for (int j = 0; j < S; ++j)
+            if (n0 + j < a.N) o[j] = (a.accumulate ? o[j] : 0.f) + a.scale * (A2[j] * LN2) * dA[j];
     }
-    if (a.dD) a.dD[row + p.d] = (a.accumulate ? a.dD[row + p.d] : 0.f) + a.scale * dD;
-    if (a.dbias) a.dbias[row + p.d] = (a.accumulate ? a.dbias[row + p.d] : 0.f) + a.scale * dbias;
+    if (sb > 0) return;
+    if (a.dD) a.dD[row + d] = (a.accumulate ? a.dD[row + d] : 0.f) + a.scale * dD;
+    if (a.dbias) a.dbias[row + d] = (a.accumulate ? a.dbias[row + d] : 0.f) + a.scale * dbias;
 }
 
 // dB and dC of all channel blocks, in their order
@@ -493,6 +703,13 @@ __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs a) {
 }
 
 int block_of(int D) { return D > 192 ? 256 : (D + 63) / 64 * 64; }
+// backward: lanes a channel's states lie on, threads of a workgroup, workgroups a row of channels needs
+int lanes_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
+int back_block_of(int D, int N) { return block_of(D > 1024 ? 1024 : D * lanes_of(N)); }
+int back_blocks_of(int D, int N) {
+    const int per = back_block_of(D, N) / lanes_of(N);
+    return (D + per - 1) / per;
+}
 
 int check(const dpk_scan_desc* s) {
     if (!s || s->B < 0 || s->T < 0 || s->D <= 0 || s->N <= 0) return DPK_EINVAL;
@@ -502,10 +719,17 @@ int check(const dpk_scan_desc* s) {
     if (s->u_sb < 0 || s->u_st < 0 || s->delta_sb < 0 || s->delta_st < 0 || s->B_sb < 0 || s->B_st < 0 || s->C_sb < 0 ||
         s->C_st < 0 || s->z_sb < 0 || s->z_st < 0)
         return DPK_EINVAL;
+    // a lane's byte offset within a group of rows is 32 bits
+    const int64_t row_limit = (int64_t)1 << 26;
+    if (s->D >= row_limit || (int64_t)s->D * s->N >= (int64_t)1 << 29 || s->u_st >= row_limit || s->delta_st >= row_limit ||
+        s->z_st >= row_limit)
+        return DPK_ERANGE;
     if (!s->A_log || (s->T > 0 && (!s->u || !s->delta || !s->Bm || !s->Cm))) return DPK_EINVAL;
     const int bl = block_of(s->D);
-    if ((int64_t)s->B * s->nchunk * ((s->D + bl - 1) / bl) > 0x7fffffffLL) return DPK_ERANGE;
-    if (((int64_t)s->B * s->N * s->D + 255) / 256 > 0x7fffffffLL) return DPK_ERANGE;
+    if ((int64_t)s->B * s->nchunk * ((s->D + bl - 1) / bl) > 0x7fffffffLL ||
+        (int64_t)s->B * s->nchunk * back_blocks_of(s->D, s->N) > 0x7fffffffLL)
+        return DPK_ERANGE;
+    if (((int64_t)s->B * s->N * s->D + 31) / 32 > 0x7fffffffLL) return DPK_ERANGE;
     return DPK_OK;
 }
 
@@ -530,17 +754,19 @@ ScanArgs fill(const dpk_scan_desc* s) {
     else if (N <= 16) { CALL(16) } \
     else { CALL(32) }
 
-// Chunks of time a scan is cut into.  A whole pass costs a second reading of the inputs and most of its arithmetic again, so it
-// has to win a factor of two in waves at least: only scans of fewer than 512 waves (half a wave a SIMD) are cut, into chunks of
-// 64 steps or more.
-extern "C" int dpk_selective_scan_chunks(int B, int T, int D, int* chunk) {
+// Chunks of time a scan is cut into.  Cutting costs a second reading of the inputs and most of the arithmetic again, so it has to
+// win a factor of two in waves at least: only scans of fewer than 512 waves (half a wave a SIMD) are cut, into up to 2048 waves.
+// Forward, chunks may be as short as 32 steps (2 x 4096 x 500, N = 16, bf16: 75 us against 102 with 64), backward 64 (145 us
+// against 154 with 32: its waves hold 16 channels, so there are four times as many to begin with).
+extern "C" int dpk_selective_scan_chunks(int B, int T, int D, int backward, int* chunk) {
     if (B <= 0 || T <= 0 || D <= 0) {
         if (chunk) *chunk = (T > 0 ? (T + GROUP - 1) / GROUP * GROUP : 0);
         return 1;
     }
     const int64_t waves = (int64_t)B * ((D + 63) / 64);
     int64_t n = waves >= 512 ? 1 : 2048 / waves;
-    const int64_t most = (T + 63) / 64;
+    const int shortest = backward ? 64 : 32;
+    const int64_t most = (T + shortest - 1) / shortest;
     if (n > most) n = most;
     if (n < 3) n = 1;
     int64_t len = (T + n - 1) / n;
@@ -551,7 +777,10 @@ extern "C" int dpk_selective_scan_chunks(int B, int T, int D, int* chunk) {
 }
 
 extern "C" int dpk_selective_scan_group(void) { return GROUP; }
-extern "C" int dpk_selective_scan_channel_blocks(int D) { return D <= 0 ? 0 : (D + block_of(D) - 1) / block_of(D); }
+extern "C" int dpk_selective_scan_state_rows(int N) { return N <= 0 || N > DPK_SCAN_MAX_STATE ? 0 : 4 * lanes_of(N); }
+extern "C" int dpk_selective_scan_channel_blocks(int D, int N) {
+    return D <= 0 || N <= 0 || N > DPK_SCAN_MAX_STATE ? 0 : back_blocks_of(D, N);
+}
 
 extern "C" int dpk_selective_scan_forward(const dpk_scan_desc* s, void* out, float* hT, void* stream) {
     const int rc = check(s);
@@ -567,7 +796,7 @@ extern "C" int dpk_selective_scan_forward(const dpk_scan_desc* s, void* out, flo
 #define CALL(NT) hipLaunchKernelGGL((scan_forward_kernel<E, NT, true>), grid, block, 0, st, a);
         DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
 #undef CALL
-        hipLaunchKernelGGL(scan_join_kernel<false>, dim3((unsigned)(((int64_t)a.nb * a.N * a.D + 255) / 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(scan_join_kernel<false>, dim3((unsigned)(((int64_t)a.nb * a.N * a.D + 31) / 32)), dim3(256), 0, st, a);
     }
 #define CALL(NT) hipLaunchKernelGGL((scan_forward_kernel<E, NT, false>), grid, block, 0, st, a);
     DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
@@ -579,13 +808,16 @@ extern "C" int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_sca
     const int rc = check(s);
     if (rc) return rc;
     if (!g || g->dout_sb < 0 || g->dout_st < 0) return DPK_EINVAL;
+    if (g->dout_st >= (int64_t)1 << 26) return DPK_ERANGE;
     if (s->B == 0) return DPK_OK;
     if (s->T > 0 && (!g->dout || !g->du || !g->ddelta || !g->dB || !g->dC || !s->kept || (s->z && !g->dz))) return DPK_EINVAL;
     if (s->nchunk > 1 && (!s->edge || !s->span)) return DPK_EINVAL;
     if ((g->dA || g->dD || g->dbias) && g->par_stride < s->D) return DPK_EINVAL;
     ScanArgs a = fill(s);
-    if (a.ndb > 1 && s->T > 0 && !g->dbc) return DPK_EINVAL;
+    const int blocks = back_blocks_of(s->D, s->N);
+    if (blocks > 1 && s->T > 0 && !g->dbc) return DPK_EINVAL;
     a.dout = g->dout; a.dhT = g->dhT; a.du = g->du; a.ddelta = g->ddelta; a.dB = g->dB; a.dC = g->dC; a.dz = s->z ? g->dz : nullptr;
+    if (!a.z) { a.z = a.u; a.z_sb = a.u_sb; a.z_st = a.u_st; }
     a.dh0 = g->dh0; a.dbc = g->dbc; a.dA = g->dA; a.dD = g->dD; a.dbias = g->dbias; a.par_stride = g->par_stride;
     a.dout_sb = g->dout_sb; a.dout_st = g->dout_st; a.scale = g->scale; a.accumulate = g->accumulate;
     const hipStream_t st = (hipStream_t)stream;
@@ -596,9 +828,11 @@ extern "C" int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_sca
 #define CALL(NT) hipLaunchKernelGGL((scan_backward_edge_kernel<E, NT>), grid, block, 0, st, a);
         DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
 #undef CALL
-        hipLaunchKernelGGL(scan_join_kernel<true>, dim3((unsigned)(((int64_t)a.nb * a.N * a.D + 255) / 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(scan_join_kernel<true>, dim3((unsigned)(((int64_t)a.nb * a.N * a.D + 31) / 32)), dim3(256), 0, st, a);
     }
-#define CALL(NT) hipLaunchKernelGGL((scan_backward_kernel<E, NT>), grid, block, 0, st, a);
+    a.ndb = blocks;
+    const dim3 bgrid((unsigned)(a.nb * a.nchunk * a.ndb)), bblock((unsigned)back_block_of(a.D, a.N));
+#define CALL(NT) hipLaunchKernelGGL((scan_backward_kernel<E, NT / 4>), bgrid, bblock, 0, st, a);
     DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
 #undef CALL
     if (a.ndb > 1 && sums > 0) {

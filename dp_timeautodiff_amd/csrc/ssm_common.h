@@ -68,14 +68,26 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // 1 / (1 + e^-x): the exponential overflows to inf for x << 0 and the reciprocal is then 0
 __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp2_hw(-x * LOG2E)); }
 
-// log(1 + e^x).  With w = fl(1 + e) the logarithm of w misses log(1 + e) by the rounding of w; (e / (w - 1)) puts it back
-// (w - 1 is exact), so small e keep their relative accuracy.  Above 20 the result is x to the last bit of fp32.
-__device__ __forceinline__ float softplus_f(float x) {
-    const float e = expf(x < 20.f ? x : 20.f);
+// log(1 + e^x) and its derivative, the sigmoid.  e^x = 2^(x log2 e): the product's rounding error, times ln 2, is put back as a
+// factor, so e keeps its relative accuracy for x << 0.  With w = fl(1 + e) the logarithm of w misses log(1 + e) by the rounding
+// of w; the factor e / (w - 1) puts that back (w - 1 is exact).  Above 20 the result is x to the last bit of fp32.
+struct Softplus {
+    float value, slope;
+};
+__device__ __forceinline__ Softplus softplus_f(float x) {
+    constexpr float LOG2E_LOW = 1.9259629911266175e-8f;   // log2 e = LOG2E + LOG2E_LOW
+    const float xc = x < 20.f ? x : 20.f;
+    const float p = xc * LOG2E;
+    const float low = __builtin_fmaf(xc, LOG2E, -p) + xc * LOG2E_LOW;
+    const float e0 = exp2_hw(p);
+    const float e = __builtin_fmaf(e0, low * LN2, e0);
     const float w = 1.f + e;
     const float d = w - 1.f;
     const float l = d == 0.f ? e : __builtin_amdgcn_logf(w) * LN2 * e * __builtin_amdgcn_rcpf(d);
-    return x < 20.f ? l : x;   // a NaN fails the comparison and comes back as itself
+    Softplus r;
+    r.value = x < 20.f ? l : x;   // a NaN fails the comparison and comes back as itself
+    r.slope = x < 20.f ? e * __builtin_amdgcn_rcpf(w) : (x == x ? 1.f : x);
+    return r;
 }
 
 template <int CTRL>

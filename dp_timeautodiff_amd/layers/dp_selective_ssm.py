@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _native
 from .dp_rnn import RNNLinear
-from .rms_norm import DPRMSNorm, _active_claim, _copy_without_runtime
+from .dp_rms_norm import DPRMSNorm, _active_claim, _copy_without_runtime
 
 _ACTIVATIONS = {None: False, "silu": True}
 

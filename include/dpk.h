@@ -372,12 +372,12 @@ int dpk_causal_conv_step(const void* x, int64_t x_sb, void* state, const float* 
  * K14: dt = softplus(delta + dt_bias) (softplus = 0: the sum itself), A = -exp(A_log) [D,N], h_t = exp(dt A) h_{t-1} + dt Bm_t u_t,
  * y = Cm_t . h_t + Dskip u_t, out = y silu(z).  u, delta, z [B,T,D], Bm, Cm [B,T,N], N <= DPK_SCAN_MAX_STATE; Dskip, z, dt_bias, h0
  * [B,D,N], lengths [B] may be NULL.  Rows at and behind lengths[b] leave the state alone and give out = 0.
- * kept: [B, ceil(T / dpk_selective_scan_group()), N, D] floats, written by forward where the backward pass is to follow (else NULL).
+ * kept: [B, ceil(T / dpk_selective_scan_group()), dpk_selective_scan_state_rows(N), D] floats, written by forward where the backward pass is to follow (else NULL).
  * nchunk, chunk: as dpk_selective_scan_chunks says (or 1 and T rounded up to the group); nchunk > 1 needs edge
  * [nchunk, B, N, D] and span [nchunk, B, D] floats of scratch, not kept between the calls.
  * backward: gradients of every input; dhT (nullable) is the gradient of the final state, dh0 (nullable) receives that of h0.
  * dA (of A_log) [D,N], dD [D], dbias [D] (each nullable): row b * nchunk + c, par_stride floats apart, receives what chunk c of sequence b
- * adds, scaled; with nchunk = 1 that is the per-sample gradient.  dbc: dpk_selective_scan_channel_blocks(D) * B * T * 2N floats where
+ * adds, scaled; with nchunk = 1 that is the per-sample gradient.  dbc: dpk_selective_scan_channel_blocks(D, N) * B * T * 2N floats where
  * that count is above 1.   step: T = 1, state [B,D,N] updated in place.
  */
 #define DPK_SCAN_MAX_STATE 32
@@ -398,9 +398,10 @@ typedef struct {
     float scale;
     int accumulate;
 } dpk_scan_grads;
-int dpk_selective_scan_chunks(int B, int T, int D, int* chunk);
+int dpk_selective_scan_chunks(int B, int T, int D, int backward, int* chunk);
 int dpk_selective_scan_group(void);
-int dpk_selective_scan_channel_blocks(int D);
+int dpk_selective_scan_state_rows(int N);
+int dpk_selective_scan_channel_blocks(int D, int N);
 int dpk_selective_scan_forward(const dpk_scan_desc* s, void* out, float* hT, void* stream);
 int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_scan_grads* g, void* stream);
 int dpk_selective_scan_step(const dpk_scan_desc* s, float* state, void* out, void* stream);

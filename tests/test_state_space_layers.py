@@ -373,9 +373,10 @@ def test_chunk_rule_covers_the_sequence():
     for B in (1, 2, 7, 64, 5000):
         for T in (0, 1, 8, 63, 64, 65, 1000, 8192, 100_003):
             for D in (1, 64, 500, 4096):
-                c = ctypes.c_int(-1)
-                n = lib.dpk_selective_scan_chunks(B, T, D, ctypes.byref(c))
-                assert n >= 1 and c.value % g == 0 and n * c.value >= T and (n - 1) * c.value < max(T, 1)
+                for back in (0, 1):
+                    c = ctypes.c_int(-1)
+                    n = lib.dpk_selective_scan_chunks(B, T, D, back, ctypes.byref(c))
+                    assert n >= 1 and c.value % g == 0 and n * c.value >= T and (n - 1) * c.value < max(T, 1)
                 s = lib.dpk_causal_conv_segments(B, T, D)
                 assert 1 <= s <= max(T, 1)
     assert lib.dpk_rms_norm_split(1, 1) == 1 and lib.dpk_rms_norm_split(0, 5) == 1
