@@ -79,7 +79,7 @@ EXPORTS = {
     "dpk_selective_scan_step": (c_int, [c_void_p] * 4),
     "dpk_compress_activation": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "dpk_restore_activation": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
-    "dpk_sum_rows": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_int64, c_float, c_int, c_void_p]),
+    "dpk_sum_rows": (c_int, [c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_float, c_int, c_void_p]),
 }
 
 
@@ -692,23 +692,24 @@ def _par(t, name: str, shape, device, dtype=torch.float32):
     return t if t.is_contiguous() else t.contiguous()
 
 
-class _on:
-    """Makes the tensors' device current for a launch and yields the stream argument."""
-    __slots__ = ("device", "guard")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent in builds of torch without a GPU runtime
 
-    def __init__(self, device):
-        self.device, self.guard = device, None
 
-    def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+def _call(name: str, device: torch.device, *args):
+    """lib.name(*args, stream) on the current stream of `device`, with that device current; raises on an error code."""
+    fn = getattr(_lib or load(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _check(rc, name)
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _as_rows(t: torch.Tensor):
@@ -725,10 +726,12 @@ def _as_btf(t: torch.Tensor):
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def sum_rows(src: torch.Tensor, groups: int, rows: int, P: int, in_stride: int, out_ptr, out_stride: int, scale: float,
-             accumulate: bool, stream):
-    _check(load().dpk_sum_rows(src if isinstance(src, c_void_p) else _ptr(src), groups, rows, P, in_stride, out_ptr, out_stride,
-                               float(scale), int(accumulate), stream), "dpk_sum_rows")
+def _sum_rows(device, src: int, groups: int, rows: int, in_stride: int, outs, scale: float, accumulate: bool):
+    """outs: up to three (address, floats, group stride) that take consecutive columns of the rows."""
+    p, n, st = (c_void_p * 3)(), (c_int64 * 3)(), (c_int64 * 3)()
+    for i, (ptr, size, stride) in enumerate(outs):
+        p[i], n[i], st[i] = ptr, size, stride
+    _call("dpk_sum_rows", device, src, groups, rows, in_stride, p, n, st, scale, int(accumulate))
 
 
 def rms_norm_forward(x, residual, weight, eps: float, want_rstd: bool, quantize: bool):
@@ -758,10 +761,8 @@ def rms_norm_forward(x, residual, weight, eps: float, want_rstd: bool, quantize:
         q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
         e = torch.empty(*x.shape[:-1], -(-C // ACT8_BLOCK), dtype=torch.uint8, device=x.device)
     if rows:
-        with _on(x.device) as stream:
-            _check(load().dpk_rms_norm_forward(_ptr(x), ld_x, _ptr(residual), ld_res, _ptr(weight), _ptr(y), _ptr(r), _ptr(rstd),
-                                               _ptr(q), _ptr(e), rows, C, float(eps), ACT_DTYPES[x.dtype], stream),
-                   "dpk_rms_norm_forward")
+        _call("dpk_rms_norm_forward", x.device, x.data_ptr(), ld_x, _addr(residual), ld_res, weight.data_ptr(), y.data_ptr(),
+              _addr(r), _addr(rstd), _addr(q), _addr(e), rows, C, eps, ACT_DTYPES[x.dtype])
     return y, r, rstd, q, e
 
 
@@ -784,22 +785,15 @@ def rms_norm_backward(r, dy, dr, weight, rstd, want_dx: bool, want_dw: bool, win
     dw = torch.empty(C, dtype=torch.float32, device=dev) if want_dw and window is None else None
     if window is not None and groups == 0:
         return dx, None
-    lib = load()
     per = rows // groups
-    split = lib.dpk_rms_norm_split(groups, per)
+    split = load().dpk_rms_norm_split(groups, per)
+    out, stride = (None, C) if not want_dw else (window.ptr.value, window.stride) if window is not None else (dw.data_ptr(), C)
     ws = torch.empty(groups * split, C, dtype=torch.float32, device=dev) if split > 1 and want_dw else None
-    with _on(dev) as stream:
-        if window is not None:
-            out, stride = window.ptr, window.stride
-        else:
-            out, stride = _ptr(dw), C
-        direct = ws is None
-        _check(lib.dpk_rms_norm_backward(_ptr(r), ld_r, _ptr(dy), ld_dy, _ptr(dr), ld_dr, _ptr(weight), _ptr(rstd), _ptr(dx),
-                                         (out if direct else _ptr(ws)) if want_dw else None, stride if direct else C, groups, per,
-                                         split, C, float(scale) if direct else 1.0, int(accumulate and direct),
-                                         ACT_DTYPES[r.dtype], stream), "dpk_rms_norm_backward")
-        if not direct:
-            sum_rows(ws, groups, split, C, C, out, stride, scale, accumulate, stream)
+    _call("dpk_rms_norm_backward", dev, r.data_ptr(), ld_r, dy.data_ptr(), ld_dy, _addr(dr), ld_dr, weight.data_ptr(),
+          rstd.data_ptr(), _addr(dx), out if ws is None else ws.data_ptr(), stride if ws is None else C, groups, per, split, C,
+          scale if ws is None else 1.0, int(accumulate and ws is None), ACT_DTYPES[r.dtype])
+    if ws is not None:
+        _sum_rows(dev, ws.data_ptr(), groups, split, C, [(out, C, stride)], scale, accumulate)
     return dx, dw
 
 
@@ -827,10 +821,8 @@ def causal_conv_forward(x, weight, bias, state, lengths, silu: bool, want_state:
     y = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
     out = torch.empty(B, W - 1, D, dtype=x.dtype, device=x.device) if want_state else None
     if B:
-        with _on(x.device) as stream:
-            _check(load().dpk_causal_conv_forward(_ptr(x), x.stride(0), x.stride(1), _ptr(weight), _ptr(bias), _ptr(state),
-                                                  _ptr(lengths), _ptr(y), _ptr(out), B, T, D, W, int(silu),
-                                                  ACT_DTYPES[x.dtype], stream), "dpk_causal_conv_forward")
+        _call("dpk_causal_conv_forward", x.device, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _addr(bias),
+              _addr(state), _addr(lengths), y.data_ptr(), _addr(out), B, T, D, W, int(silu), ACT_DTYPES[x.dtype])
     return y, out
 
 
@@ -849,35 +841,33 @@ def causal_conv_backward(x, weight, bias, state, lengths, silu: bool, dy, dstate
     dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
     dstate = torch.empty(B, W - 1, D, dtype=x.dtype, device=dev) if want_dstate else None
     nb = 0 if bias is None else D
-    flat = torch.empty(D * W + nb, dtype=torch.float32, device=dev) if want_par and windows is None else None
-    lib = load()
-    seg = lib.dpk_causal_conv_segments(B, T, D)
+    grads = None
+    if want_par and windows is None:
+        grads = (torch.empty(D, W, dtype=torch.float32, device=dev),
+                 torch.empty(D, dtype=torch.float32, device=dev) if nb else None)
+    seg = load().dpk_causal_conv_segments(B, T, D)
     ww, wb = windows if windows is not None else (None, None)
     if ww is not None and (ww.numel != D * W or ww.base.shape[0] < B or (wb is None) != (bias is None)
                            or (wb is not None and wb.numel != D)):
         raise DpkError("causal_conv: grad-sample windows do not match the layer")
-    direct = ww is not None and seg == 1   # one segment: the kernel's row is the sample's arena row
+    # one segment: the kernel's row is the sample's arena row, the bias window somewhere behind the weight's
+    direct = ww is not None and seg == 1 and (wb is None or wb.offset >= ww.offset)
+    ws, par, stride, off = None, None, 0, -1
     if direct:
-        par, stride, off = ww.ptr, ww.stride, (wb.offset - ww.offset if wb is not None else -1)
-        direct = wb is None or off >= 0
-    ws = None
-    if want_par and not direct:
+        par, stride, off = ww.ptr.value, ww.stride, (wb.offset - ww.offset if wb is not None else -1)
+    elif want_par:
         ws = torch.empty(max(B * seg, 1), D * W + nb, dtype=torch.float32, device=dev)
-        par, stride, off = _ptr(ws), D * W + nb, (D * W if nb else -1)
-    with _on(dev) as stream:
-        if B:
-            _check(lib.dpk_causal_conv_backward(
-                _ptr(x), x.stride(0), x.stride(1), _ptr(dy), dy.stride(0), dy.stride(1), _ptr(weight), _ptr(bias), _ptr(state),
-                _ptr(dstate_out), _ptr(lengths), _ptr(dx), _ptr(dstate), par if want_par else None, stride if want_par else 0,
-                off if want_par else -1, seg, B, T, D, W, int(silu), float(scale) if direct else 1.0, int(accumulate and direct),
-                ACT_DTYPES[x.dtype], stream), "dpk_causal_conv_backward")
-        if flat is not None:
-            sum_rows(ws, 1, B * seg, D * W + nb, D * W + nb, _ptr(flat), D * W + nb, scale, False, stream)
-        elif ws is not None and B:
-            sum_rows(ws, B, seg, D * W, stride, ww.ptr, ww.stride, scale, accumulate, stream)
-            if wb is not None:
-                sum_rows(c_void_p(ws.data_ptr() + 4 * D * W), B, seg, D, stride, wb.ptr, wb.stride, scale, accumulate, stream)
-    grads = None if flat is None else (flat[:D * W].view(D, W), flat[D * W:] if nb else None)
+        par, stride, off = ws.data_ptr(), D * W + nb, (D * W if nb else -1)
+    if B:
+        _call("dpk_causal_conv_backward", dev, x.data_ptr(), x.stride(0), x.stride(1), dy.data_ptr(), dy.stride(0), dy.stride(1),
+              weight.data_ptr(), _addr(bias), _addr(state), _addr(dstate_out), _addr(lengths), dx.data_ptr(), _addr(dstate), par,
+              stride, off, seg, B, T, D, W, int(silu), scale if direct else 1.0, int(accumulate and direct), ACT_DTYPES[x.dtype])
+    if grads is not None:
+        outs = [(g.data_ptr(), g.numel(), g.numel()) for g in grads if g is not None]
+        _sum_rows(dev, ws.data_ptr(), 1, B * seg, stride, outs, scale, False)
+    elif ws is not None and B:
+        _sum_rows(dev, ws.data_ptr(), B, seg, stride, [(w.ptr.value, w.numel, w.stride) for w in (ww, wb) if w is not None], scale,
+                  accumulate)
     return dx, dstate, grads
 
 
@@ -899,9 +889,8 @@ def causal_conv_step(x, state, weight, bias, silu: bool):
         x = x.contiguous()
     y = torch.empty(B, D, dtype=x.dtype, device=x.device)
     if B:
-        with _on(x.device) as stream:
-            _check(load().dpk_causal_conv_step(_ptr(x), x.stride(0), _ptr(state), _ptr(weight), _ptr(bias), _ptr(y), B, D, W,
-                                               int(silu), ACT_DTYPES[x.dtype], stream), "dpk_causal_conv_step")
+        _call("dpk_causal_conv_step", x.device, x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _addr(bias),
+              y.data_ptr(), B, D, W, int(silu), ACT_DTYPES[x.dtype])
     return y
 
 
@@ -945,29 +934,35 @@ class ScanInputs:
         self.lengths = _par(lengths, "lengths", (u.shape[0],), dev, torch.int32)
         self.softplus = bool(softplus)
 
+    @classmethod
+    def checked(cls, u, delta, A_log, B, C, D, z, dt_bias, h0, lengths, softplus):
+        """Operands that a ScanInputs has held before."""
+        self = cls.__new__(cls)
+        self.u, self.delta, self.A_log, self.B, self.C, self.D, self.z, self.dt_bias = u, delta, A_log, B, C, D, z, dt_bias
+        self.h0, self.lengths, self.softplus = h0, lengths, softplus
+        return self
+
     def desc(self, kept=None, backward: bool = False):
         """dpk_scan_desc and the scratch it points at."""
-        u = self.u
-        b, t = (u.shape[0], u.shape[1]) if u.dim() == 3 else (u.shape[0], 1)
+        u, delta, B, C, z = self.u, self.delta, self.B, self.C, self.z
         d, n = self.A_log.shape
-        chunk = c_int(0)
-        nchunk = load().dpk_selective_scan_chunks(b, t, d, int(backward), ctypes.byref(chunk)) if u.dim() == 3 else 1
-        s = _ScanDesc()
-        s.B, s.T, s.D, s.N, s.softplus, s.dtype = b, t, d, n, int(self.softplus), ACT_DTYPES[u.dtype]
-        s.nchunk, s.chunk = nchunk, chunk.value if u.dim() == 3 else load().dpk_selective_scan_group()
-        for name, x in (("u", u), ("delta", self.delta), ("Bm", self.B), ("Cm", self.C), ("z", self.z), ("A_log", self.A_log),
-                        ("Dskip", self.D), ("dt_bias", self.dt_bias), ("h0", self.h0), ("lengths", self.lengths), ("kept", kept)):
-            setattr(s, name, None if x is None else x.data_ptr())
-        for name, x in (("u", u), ("delta", self.delta), ("B", self.B), ("C", self.C), ("z", self.z)):
-            if x is not None:
-                setattr(s, name + "_sb", x.stride(0))
-                setattr(s, name + "_st", x.stride(1) if x.dim() == 3 else 0)
-        scratch = None
-        if nchunk > 1:
-            scratch = torch.empty(nchunk * b * (n + 1) * d, dtype=torch.float32, device=u.device)
-            s.edge = scratch.data_ptr()
-            s.span = scratch.data_ptr() + 4 * nchunk * b * n * d
-        return s, scratch
+        lib = load()
+        scratch = edge = span = None
+        if u.dim() == 3:
+            b, t, _ = u.shape
+            chunk = c_int(0)
+            nchunk, chunk = lib.dpk_selective_scan_chunks(b, t, d, int(backward), ctypes.byref(chunk)), chunk.value
+            if nchunk > 1:
+                scratch = torch.empty(nchunk * b * (n + 1) * d, dtype=torch.float32, device=u.device)
+                edge = scratch.data_ptr()
+                span = edge + 4 * nchunk * b * n * d
+            strides = (*u.stride()[:2], *delta.stride()[:2], *B.stride()[:2], *C.stride()[:2], *((0, 0) if z is None else z.stride()[:2]))
+        else:
+            b, t, nchunk, chunk = u.shape[0], 1, 1, lib.dpk_selective_scan_group()
+            strides = (u.stride(0), 0, delta.stride(0), 0, B.stride(0), 0, C.stride(0), 0, 0 if z is None else z.stride(0), 0)
+        return _ScanDesc(u.data_ptr(), delta.data_ptr(), B.data_ptr(), C.data_ptr(), _addr(z), self.A_log.data_ptr(), _addr(self.D),
+                         _addr(self.dt_bias), _addr(self.h0), _addr(self.lengths), _addr(kept), edge, span, *strides, b, t, d, n,
+                         self.softplus, nchunk, chunk, ACT_DTYPES[u.dtype]), scratch
 
 
 def selective_scan_forward(inp: ScanInputs, want_kept: bool, want_state: bool):
@@ -982,9 +977,8 @@ def selective_scan_forward(inp: ScanInputs, want_kept: bool, want_state: bool):
     kept = torch.empty(b, (t + g - 1) // g, lib.dpk_selective_scan_state_rows(n), d, dtype=torch.float32,
                        device=u.device) if want_kept else None
     if b:
-        with _on(u.device) as stream:
-            s, scratch = inp.desc(kept)
-            _check(lib.dpk_selective_scan_forward(ctypes.byref(s), _ptr(out), _ptr(hT), stream), "dpk_selective_scan_forward")
+        s, scratch = inp.desc(kept)
+        _call("dpk_selective_scan_forward", u.device, ctypes.byref(s), out.data_ptr(), _addr(hT))
     return out, hT, kept
 
 
@@ -999,47 +993,44 @@ def selective_scan_backward(inp: ScanInputs, kept, dout, dhT, want_dh0: bool, wa
     _act(dout, "dout", u.shape, u)
     dout = dout if dout.stride(2) == 1 or d == 1 else dout.contiguous()
     dhT = _par(dhT, "dstate", (b, d, n), dev)
-    new = lambda *shape: torch.empty(*shape, dtype=u.dtype, device=dev)  # noqa: E731
-    du, ddelta, dB, dC = new(b, t, d), new(b, t, d), new(b, t, n), new(b, t, n)
-    dz = new(b, t, d) if inp.z is not None else None
+    new = u.new_empty
+    du, ddelta, dB, dC = new(u.shape), new(u.shape), new((b, t, n)), new((b, t, n))
+    dz = new(u.shape) if inp.z is not None else None
     dh0 = torch.empty(b, d, n, dtype=torch.float32, device=dev) if want_dh0 else None
     P = d * (n + 2)
-    flat = torch.empty(P, dtype=torch.float32, device=dev) if want_par and windows is None else None
+    grads = None
     if windows is not None:
         for w, size in zip(windows, (d * n, d, d)):
             if w is not None and (w.numel != size or w.base.shape[0] < b):
                 raise DpkError("selective_scan: grad-sample windows do not match the layer")
-    lib = load()
-    if b:
-        with _on(dev) as stream:
-            s, scratch = inp.desc(kept, True)
-            g = _ScanGrads()
-            g.dout, g.dout_sb, g.dout_st = dout.data_ptr(), dout.stride(0), dout.stride(1)
-            for name, x in (("dhT", dhT), ("du", du), ("ddelta", ddelta), ("dB", dB), ("dC", dC), ("dz", dz), ("dh0", dh0)):
-                setattr(g, name, None if x is None else x.data_ptr())
-            blocks = lib.dpk_selective_scan_channel_blocks(d, n)
-            dbc = torch.empty(blocks, b, t, 2 * n, dtype=torch.float32, device=dev) if blocks > 1 else None
-            g.dbc = None if dbc is None else dbc.data_ptr()
-            direct = windows is not None and s.nchunk == 1
-            ws = None
-            g.scale, g.accumulate = 1.0, 0
-            if want_par and direct:
-                g.dA, g.dD, g.dbias = (None if w is None else w.ptr.value for w in windows)
-                g.par_stride, g.scale, g.accumulate = windows[0].stride, float(scale), int(accumulate)
-            elif want_par:
-                ws = torch.empty(b * s.nchunk, P, dtype=torch.float32, device=dev)
-                g.dA, g.dD, g.dbias = ws.data_ptr(), ws.data_ptr() + 4 * d * n, ws.data_ptr() + 4 * d * (n + 1)
-                g.par_stride = P
-            _check(lib.dpk_selective_scan_backward(ctypes.byref(s), ctypes.byref(g), stream), "dpk_selective_scan_backward")
-            if flat is not None:
-                sum_rows(ws, 1, b * s.nchunk, P, P, _ptr(flat), P, scale, False, stream)
-            elif ws is not None:
-                for w, off, size in zip(windows, (0, d * n, d * (n + 1)), (d * n, d, d)):
-                    if w is not None:
-                        sum_rows(c_void_p(ws.data_ptr() + 4 * off), b, s.nchunk, size, P, w.ptr, w.stride, scale, accumulate, stream)
-    elif flat is not None:
-        flat.zero_()
-    grads = None if flat is None else (flat[:d * n].view(d, n), flat[d * n:d * (n + 1)], flat[d * (n + 1):])
+    elif want_par:
+        make = torch.empty if b else torch.zeros
+        grads = tuple(make(size, dtype=torch.float32, device=dev) for size in ((d, n), (d,), (d,)))
+    if b == 0:
+        return du, ddelta, dB, dC, dz, dh0, grads
+    s, scratch = inp.desc(kept, True)
+    blocks = load().dpk_selective_scan_channel_blocks(d, n)
+    dbc = torch.empty(blocks * b * t * 2 * n, dtype=torch.float32, device=dev) if blocks > 1 else None
+    direct = windows is not None and s.nchunk == 1
+    ws, par, stride = None, (None, None, None), 0
+    if direct:
+        par, stride = tuple(None if w is None else w.ptr.value for w in windows), windows[0].stride
+    elif want_par:
+        ws = torch.empty(b * s.nchunk * P, dtype=torch.float32, device=dev)
+        p = ws.data_ptr()
+        par, stride = (p, p + 4 * d * n, p + 4 * d * (n + 1)), P
+    g = _ScanGrads(dout.data_ptr(), _addr(dhT), du.data_ptr(), ddelta.data_ptr(), dB.data_ptr(), dC.data_ptr(), _addr(dz), _addr(dh0),
+                   _addr(dbc), *par, dout.stride(0), dout.stride(1), stride, scale if direct else 1.0, int(accumulate and direct))
+    _call("dpk_selective_scan_backward", dev, ctypes.byref(s), ctypes.byref(g))
+    if grads is not None:
+        _sum_rows(dev, p, 1, b * s.nchunk, P, [(x.data_ptr(), x.numel(), x.numel()) for x in grads], scale, False)
+    elif ws is not None:   # columns of absent parameters are skipped over
+        if windows[1] is not None and windows[2] is not None:
+            _sum_rows(dev, p, b, s.nchunk, P, [(w.ptr.value, w.numel, w.stride) for w in windows], scale, accumulate)
+        else:
+            for w, off in zip(windows, (0, d * n, d * (n + 1))):
+                if w is not None:
+                    _sum_rows(dev, p + 4 * off, b, s.nchunk, P, [(w.ptr.value, w.numel, w.stride)], scale, accumulate)
     return du, ddelta, dB, dC, dz, dh0, grads
 
 
@@ -1051,9 +1042,8 @@ def selective_scan_step(inp: ScanInputs, state):
         raise DpkError("selective_scan_step: the state is updated in place and must be a contiguous [B, D, N]")
     out = torch.empty(b, d, dtype=u.dtype, device=u.device)
     if b:
-        with _on(u.device) as stream:
-            s, _ = inp.desc()
-            _check(load().dpk_selective_scan_step(ctypes.byref(s), _ptr(state), _ptr(out), stream), "dpk_selective_scan_step")
+        s, _ = inp.desc()
+        _call("dpk_selective_scan_step", u.device, ctypes.byref(s), state.data_ptr(), out.data_ptr())
     return out
 
 
@@ -1067,9 +1057,8 @@ def compress_activation(x):
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     e = torch.empty(*x.shape[:-1], -(-C // ACT8_BLOCK), dtype=torch.uint8, device=x.device)
     if x.numel():
-        with _on(x.device) as stream:
-            _check(load().dpk_compress_activation(_ptr(x), ld, _ptr(q), _ptr(e), x.numel() // C, C, ACT_DTYPES[x.dtype], stream),
-                   "dpk_compress_activation")
+        _call("dpk_compress_activation", x.device, x.data_ptr(), ld, q.data_ptr(), e.data_ptr(), x.numel() // C, C,
+              ACT_DTYPES[x.dtype])
     return q, e
 
 
@@ -1084,7 +1073,5 @@ def restore_activation(q, e, dtype):
         raise DpkError("restore_activation: data and exponents must be contiguous")
     x = torch.empty(q.shape, dtype=dtype, device=q.device)
     if q.numel():
-        with _on(q.device) as stream:
-            _check(load().dpk_restore_activation(_ptr(q), _ptr(e), _ptr(x), q.numel() // C, C, ACT_DTYPES[dtype], stream),
-                   "dpk_restore_activation")
+        _call("dpk_restore_activation", q.device, q.data_ptr(), e.data_ptr(), x.data_ptr(), q.numel() // C, C, ACT_DTYPES[dtype])
     return x

@@ -144,44 +144,55 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256)
         for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
     }
     const float inv_c = 1.f / (float)C;
-    int parity = 0;
-    for (int64_t r0 = lo; r0 < hi; r0 += RPB, parity ^= 1) {
-        const bool live = r0 + slot < hi;
-        const int64_t row = group * rows_per_group + (live ? r0 + slot : lo);
-        const float rstd = RSTD[row];
-        float x[K][V], g[K][V];
-        float dot = 0.f;
+    // two rows of a slot are under way where they fit the registers: 16 bytes a lane and row are too few to fill HBM's latency
+    constexpr int NR = E <= 8 ? 2 : 1;
+    for (int64_t r0 = lo; r0 < hi; r0 += RPB * NR) {
+        float x[NR][K][V], g[NR][K][V], d[NR][K][V], rstd[NR], dot[NR];
+        bool live[NR];
+        int64_t row[NR];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * LPR + lane) * V;
-            const int n = live && c < C ? C - c : 0;
-            load_n<T, V>(R + row * ld_r + c, n, x[k]);
-            load_n<T, V>(DY + row * ld_dy + c, n, g[k]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                x[k][i] *= rstd;
-                dw[k][i] += g[k][i] * x[k][i];
-                g[k][i] *= w[k][i];
-                dot += g[k][i] * x[k][i];
-            }
-        }
-        dot = row_sum<LPR>(dot, red, parity) * inv_c;
-        if (DX) {
+        for (int j = 0; j < NR; ++j) {
+            live[j] = r0 + j * RPB + slot < hi;
+            row[j] = group * rows_per_group + (live[j] ? r0 + j * RPB + slot : lo);
+            rstd[j] = RSTD[row[j]];
+            dot[j] = 0.f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int c = (k * LPR + lane) * V;
-                const int n = live && c < C ? C - c : 0;
-                float d[V];
-                if (DR) {
-                    load_n<T, V>(DR + row * ld_dr + c, n, d);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] += rstd * (g[k][i] - x[k][i] * dot);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] = rstd * (g[k][i] - x[k][i] * dot);
-                }
-                store_n<T, V>(DX + row * C + c, n, d);
+                const int n = live[j] && c < C ? C - c : 0;
+                load_n<T, V>(R + row[j] * ld_r + c, n, x[j][k]);
+                load_n<T, V>(DY + row[j] * ld_dy + c, n, g[j][k]);
+                if (DX && DR) load_n<T, V>(DR + row[j] * ld_dr + c, n, d[j][k]);
             }
+        }
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[j][k][i] *= rstd[j];
+                    dw[k][i] += g[j][k][i] * x[j][k][i];
+                    g[j][k][i] *= w[k][i];
+                    dot[j] += g[j][k][i] * x[j][k][i];
+                }
+            dot[j] = row_sum<LPR>(dot[j], red, NR == 2 ? j : (int)((r0 - lo) / RPB & 1)) * inv_c;
+        }
+        if (DX) {
+#pragma unroll
+            for (int j = 0; j < NR; ++j)
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const int c = (k * LPR + lane) * V;
+                    const int n = live[j] && c < C ? C - c : 0;
+                    float o[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        o[i] = rstd[j] * (g[j][k][i] - x[j][k][i] * dot[j]);
+                        if (DR) o[i] += d[j][k][i];
+                    }
+                    store_n<T, V>(DX + row[j] * C + c, n, o);
+                }
         }
     }
     if (!DW) return;

@@ -73,17 +73,19 @@ __device__ __forceinline__ void stage_bc(const ScanArgs& a, int b, int t0, int e
     }
 }
 
-// The same in two halves: fetched into registers, put into LDS once the group before is done with its half of the buffer.
+// The same in two halves, for workgroups of 256: fetched into registers, put into LDS once the group before is done with its half
+// of the buffer.  (Smaller workgroups, of narrow layers, stage in one go.)
 template <int NT>
 struct Staged {
-    static constexpr int K = GROUP * 2 * NT / 64;   // a workgroup of one wave takes all K turns
+    static constexpr int K = GROUP * 2 * NT > 256 ? GROUP * 2 * NT / 256 : 1;
     float v[K];
 };
 template <typename T, int NT>
 __device__ __forceinline__ void fetch_bc(const ScanArgs& a, int b, int t0, int end, Staged<NT>& r) {
+    if (blockDim.x != 256) return;
 #pragma unroll
     for (int k = 0; k < Staged<NT>::K; ++k) {
-        const int i = threadIdx.x + k * blockDim.x;
+        const int i = threadIdx.x + k * 256;
         const int q = i / (2 * NT), c = i % (2 * NT), n = c % NT;
         r.v[k] = 0.f;
         if (i < GROUP * 2 * NT && t0 + q < end && n < a.N)
@@ -91,11 +93,15 @@ __device__ __forceinline__ void fetch_bc(const ScanArgs& a, int b, int t0, int e
                             : to_f32(((const T*)a.C)[(int64_t)b * a.C_sb + (int64_t)(t0 + q) * a.C_st + n]);
     }
 }
-template <int NT>
-__device__ __forceinline__ void put_bc(const Staged<NT>& r, float (&s)[GROUP][2 * NT]) {
+template <typename T, int NT>
+__device__ __forceinline__ void put_bc(const ScanArgs& a, int b, int t0, int end, const Staged<NT>& r, float (&s)[GROUP][2 * NT]) {
+    if (blockDim.x != 256) {
+        stage_bc<T, NT>(a, b, t0, end, s);
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < Staged<NT>::K; ++k) {
-        const int i = threadIdx.x + k * blockDim.x;
+        const int i = threadIdx.x + k * 256;
         if (i < GROUP * 2 * NT) (&s[0][0])[i] = r.v[k];
     }
 }
@@ -413,16 +419,23 @@ __device__ __forceinline__ void spread(const float (&own)[GROUP / LS], float (&a
         }
     }
 }
-// The sums over a channel's lanes, each step's at its owner; leaves them in all[0 .. GROUP / LS).
+// The sums over a channel's lanes, each step's at its owner; leaves them in all[0 .. GROUP / LS).  The first halving pairs steps q
+// and q + GROUP / 2 (pair), as soon as both are there.
+template <int LS>
+__device__ __forceinline__ void pair(float (&all)[GROUP], int q) {
+    if constexpr (LS >= 2) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(all[q]), __float_as_uint(all[q + GROUP / 2]), false, false);
+        all[q] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+}
 template <int LS>
 __device__ __forceinline__ void collect(float (&all)[GROUP]) {
-    if constexpr (LS >= 2) fold32<GROUP>(all);
     if constexpr (LS >= 4) fold16<GROUP / 2>(all);
     if constexpr (LS >= 8) fold_dpp<GROUP / 4, 0x128, 8>(all);
 }
 
 template <typename T, int LS>
-__global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(ScanArgs a) {
     constexpr int S = 4, NT = S * LS, CPW = 64 / LS, OWN = GROUP / LS;
     __shared__ float bc[2][GROUP][2 * NT];
     __shared__ float part[2][4][GROUP][2 * NT];
@@ -459,9 +472,6 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
     // branch round it and a wait for it, in the middle of the arithmetic that is to hide it.)
     float nu[OWN], npre[OWN], ndy[OWN], nz[OWN], nh[S];
     Staged<NT> nbc;
-    const uint32_t first = (uint32_t)dd * sizeof(T);
-    const uint32_t lane_u = (uint32_t)(q0 * a.u_st + dd) * sizeof(T), lane_pre = (uint32_t)(q0 * a.delta_st + dd) * sizeof(T);
-    const uint32_t lane_dy = (uint32_t)(q0 * a.dout_st + dd) * sizeof(T), lane_z = (uint32_t)(q0 * a.z_st + dd) * sizeof(T);
     const uint32_t lane_out = ((uint32_t)q0 * a.D + d) * sizeof(T);
     const bool gate = a.dz != nullptr;   // without a gate a.z is a.u: read, and not used
     const uint32_t lane_kept = ((uint32_t)n0 * a.D + dd) * 4u;
@@ -470,14 +480,15 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
         const char* gd = group_row<T>(a.delta, a.delta_sb, a.delta_st, b, t0);
         const char* go = group_row<T>(a.dout, a.dout_sb, a.dout_st, b, t0);
         const char* gz = group_row<T>(a.z, a.z_sb, a.z_st, b, t0);
+        uint32_t q = q0;
+        asm volatile("" : "+v"(q));   // offsets are made here: held over the group they would be spilled, and waited for
 #pragma unroll
         for (int i = 0; i < OWN; ++i) {
-            const bool in = t0 + q0 + i < end;
-            const uint32_t es = (uint32_t)i * sizeof(T);
-            nu[i] = at<T>(gu, in ? lane_u + es * (uint32_t)a.u_st : first);
-            npre[i] = at<T>(gd, in ? lane_pre + es * (uint32_t)a.delta_st : first);
-            ndy[i] = at<T>(go, in ? lane_dy + es * (uint32_t)a.dout_st : first);
-            nz[i] = at<T>(gz, in ? lane_z + es * (uint32_t)a.z_st : first);
+            const uint32_t r = (int)(t0 + q + i) < end ? q + i : 0u;
+            nu[i] = at<T>(gu, (r * (uint32_t)a.u_st + dd) * (uint32_t)sizeof(T));
+            npre[i] = at<T>(gd, (r * (uint32_t)a.delta_st + dd) * (uint32_t)sizeof(T));
+            ndy[i] = at<T>(go, (r * (uint32_t)a.dout_st + dd) * (uint32_t)sizeof(T));
+            nz[i] = at<T>(gz, (r * (uint32_t)a.z_st + dd) * (uint32_t)sizeof(T));
         }
         const char* k = (const char*)(a.kept + ((int64_t)b * ngroup + t0 / GROUP) * NT * a.D);
 #pragma unroll
@@ -510,7 +521,7 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
     if (t0 >= lo) {
         fetch(t0);
         fetch_bc<T, NT>(a, b, t0, end, nbc);
-        put_bc<NT>(nbc, bc[0]);
+        put_bc<T, NT>(a, b, t0, end, nbc, bc[0]);
         __syncthreads();
     }
     for (; t0 >= lo; t0 -= GROUP) {
@@ -518,6 +529,8 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
         float dt[GROUP], x[GROUP], g[GROUP], into[GROUP], along[GROUP], y[GROUP];
         float e[GROUP][S], eh[GROUP][S];   // decay, and what it leaves of the state before the step
         const int next = t0 - GROUP >= lo ? t0 - GROUP : t0;   // (the first group is fetched twice)
+        uint32_t to = lane_out;
+        asm volatile("" : "+v"(to));
         fetch_bc<T, NT>(a, b, next, end, nbc);
         {
             float xs[OWN];
@@ -546,6 +559,7 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
             for (int j = 0; j < S; ++j) h[j] = n0 + j < a.N && live ? nh[j] : 0.f;
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
+                __builtin_amdgcn_sched_barrier(0);
                 float v[S];
                 y[q] = 0.f;
 #pragma unroll
@@ -556,7 +570,8 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
                     y[q] += bc[ph][q][NT + n0 + j] * h[j];
                     v[j] = g[q] * h[j];
                 }
-                part[ph][wave][q][NT + part_slot] = lane_sums<LS>(v);   // lanes that hold the same sum write it to the same place
+                part[ph][wave][q][NT + part_slot] = lane_sums<LS>(v);
+                if (q >= GROUP / 2) pair<LS>(y, q - GROUP / 2);   // lanes that hold the same sum write it to the same place
             }
         }
         collect<LS>(y);
@@ -565,12 +580,13 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
             for (int i = 0; i < OWN; ++i) {
                 const int t = t0 + q0 + i;
                 if (live && t < hi)
-                    put<T>((char*)a.dz + ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T), lane_out, t < end ? zf[i] * (y[i] + skip * u[i]) : 0.f);
+                    put<T>((char*)a.dz + ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T), to, t < end ? zf[i] * (y[i] + skip * u[i]) : 0.f);
             }
         }
         asm volatile("" ::: "memory");   // B and C are read from LDS again rather than held for all steps
 #pragma unroll
         for (int q = GROUP - 1; q >= 0; --q) {
+            __builtin_amdgcn_sched_barrier(0);
             // half of the group's registers are free again: the next group's operands come in behind the other half
             if (q == GROUP / 2 - 1) fetch(next);
             float v[S];
@@ -587,13 +603,17 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
                 asm volatile("" : "+v"(dA[j]));   // summed here, not behind the group with eight steps' t held until then
             }
             part[ph][wave][q][part_slot] = lane_sums<LS>(v);
+            if (q < GROUP / 2) {
+                pair<LS>(into, q);
+                pair<LS>(along, q);
+            }
         }
         // Wait for the next group's operands here, before this group's stores: a wait behind them would be one for them as well.
 #pragma unroll
         for (int i = 0; i < OWN; ++i) asm volatile("" : "+v"(nu[i]), "+v"(npre[i]), "+v"(ndy[i]), "+v"(nz[i]));
 #pragma unroll
         for (int j = 0; j < S; ++j) asm volatile("" : "+v"(nh[j]));
-        put_bc<NT>(nbc, bc[ph ^ 1]);
+        put_bc<T, NT>(a, b, next, end, nbc, bc[ph ^ 1]);
         collect<LS>(into);
         collect<LS>(along);
 #pragma unroll
@@ -604,8 +624,8 @@ __global__ void __launch_bounds__(256, 2) scan_backward_kernel(ScanArgs a) {
             if (in) dbias += dpre;
             if (live && t < hi) {
                 const int64_t o = ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T);
-                put<T>((char*)a.du + o, lane_out, in ? into[i] * dts[i] + skip * gs[i] : 0.f);
-                put<T>((char*)a.ddelta + o, lane_out, in ? dpre : 0.f);
+                put<T>((char*)a.du + o, to, in ? into[i] * dts[i] + skip * gs[i] : 0.f);
+                put<T>((char*)a.ddelta + o, to, in ? dpre : 0.f);
             }
         }
         __syncthreads();   // the group's sums are written, the next group's B and C staged

@@ -42,6 +42,8 @@ __device__ __forceinline__ void load_n(const T* __restrict__ p, int n, float (&f
     }
 }
 
+// Results leave past the caches: what they would push out is the inputs that other workgroups are about to read (a convolution
+// over 8 x 4096 x 1024 in bf16: 46 us with plain stores, 32 so; norm 317 -> 307, 8-bit round trip 195 -> 179).
 template <typename T, int V>
 __device__ __forceinline__ void store_n(T* __restrict__ p, int n, const float (&f)[V]) {
     if (n >= V) {
@@ -52,7 +54,7 @@ __device__ __forceinline__ void store_n(T* __restrict__ p, int n, const float (&
         } x;
 #pragma unroll
         for (int i = 0; i < V; ++i) x.e[i] = (T)f[i];
-        *reinterpret_cast<typename Words<(int)sizeof(T), W>::type*>(p) = x.w;
+        __builtin_nontemporal_store(x.w, reinterpret_cast<typename Words<(int)sizeof(T), W>::type*>(p));
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)

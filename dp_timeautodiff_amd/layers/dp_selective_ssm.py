@@ -92,7 +92,7 @@ class _SelectiveScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout, dstate=None):
         *operands, kept = ctx.saved_tensors
-        inp = _native.ScanInputs(*operands, ctx.softplus)
+        inp = _native.ScanInputs.checked(*operands, ctx.softplus)
         need = ctx.needs_input_grad
         if dout is None:
             dout = torch.zeros_like(inp.u)

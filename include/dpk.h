@@ -410,12 +410,14 @@ int dpk_selective_scan_step(const dpk_scan_desc* s, float* state, void* out, voi
  * K15: X [rows, C] (row stride ld_x) as Q int8 [rows, C] and one exponent byte per block of 128 elements of a row, QE [rows,
  * ceil(C/128)]: with k the least integer >= -126 such that max|x| <= 127 * 2^k, q = rint(x * 2^-k) and the byte is k + 127 (at k = 122 |q| is
  * held to 63, so that no finite value restores as inf).  A block that holds an inf or NaN has the byte 255 and restores as NaN.  restore writes q * 2^k in any dtype.
- * dpk_sum_rows: out[g][c] (+)= scale * sum_r in[g][r][c] in a fixed order (joins the partial parameter gradients of K12..K14).
+ * dpk_sum_rows: scale * sum_r in[g][r][c] in a fixed order, rows of in_stride floats; the first n[0] columns go (or are added) to
+ * out[0] + g * out_stride[0], the next n[1] to out[1], the next n[2] to out[2] (host arrays of three; n = 0: none).  Joins the
+ * partial parameter gradients of K12..K14.
  */
 int dpk_compress_activation(const void* X, int64_t ld_x, int8_t* Q, uint8_t* QE, int64_t rows, int C, int dtype, void* stream);
 int dpk_restore_activation(const int8_t* Q, const uint8_t* QE, void* X, int64_t rows, int C, int dtype, void* stream);
-int dpk_sum_rows(const float* in, int groups, int rows, int64_t P, int64_t in_stride, float* out, int64_t out_stride,
-                 float scale, int accumulate, void* stream);
+int dpk_sum_rows(const float* in, int groups, int rows, int64_t in_stride, float* const* out, const int64_t* n,
+                 const int64_t* out_stride, float scale, int accumulate, void* stream);
 
 #ifdef __cplusplus
 }

@@ -149,6 +149,8 @@ class _ScanInputs:
         self.u, self.delta, self.A_log, self.B, self.C, self.D, self.z, self.dt_bias = u, delta, A_log, B, C, D, z, dt_bias
         self.h0, self.lengths, self.softplus = h0, lengths, softplus
 
+    checked = classmethod(lambda cls, *a: cls(*a))
+
     def tensors(self, rows=slice(None)):
         cut = lambda t: None if t is None else t[rows]  # noqa: E731
         return cut(self.u), cut(self.delta), self.A_log, cut(self.B), cut(self.C), self.D, cut(self.z), self.dt_bias, cut(self.h0)

@@ -360,7 +360,11 @@ def test_c_entry_refusals():
     assert lib.dpk_selective_scan_backward(ctypes.byref(scan()), None, None) == -1 and lib.dpk_selective_scan_forward(None, p, None, None) == -1
     assert lib.dpk_selective_scan_step(ctypes.byref(scan()), p, p, None) == -1   # T is not 1
     assert lib.dpk_compress_activation(None, 8, p, p, 4, 8, 0, None) == lib.dpk_compress_activation(p, 8, p, p, 4, 0, 0, None) == -1
-    assert lib.dpk_restore_activation(p, p, p, 4, 8, 7, None) == -1 and lib.dpk_sum_rows(p, 1, 4, 8, 7, p, 8, 1.0, 0, None) == -1
+    assert lib.dpk_restore_activation(p, p, p, 4, 8, 7, None) == -1
+    out, n, st = (ctypes.c_void_p * 3)(4096, None, None), (ctypes.c_int64 * 3)(8, 0, 0), (ctypes.c_int64 * 3)(8, 0, 0)
+    assert lib.dpk_sum_rows(p, 1, 4, 7, out, n, st, 1.0, 0, None) == lib.dpk_sum_rows(p, 1, 4, 8, out, None, st, 1.0, 0, None) == -1
+    n[1] = 3   # columns without a destination
+    assert lib.dpk_sum_rows(p, 1, 4, 16, out, n, st, 1.0, 0, None) == -1
     # and what is empty is done
     assert norm(**ok(rows=0)) == 0 and lib.dpk_compress_activation(None, 8, None, None, 0, 8, 0, None) == 0 and fwd(B=0) == 0
 
