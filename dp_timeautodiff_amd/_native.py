@@ -689,7 +689,7 @@ def _par(t, name: str, shape, device, dtype=torch.float32):
     _req(t, name, dtype)
     if tuple(t.shape) != tuple(shape) or t.device != device:
         raise DpkError(f"{name}: expected shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
-    return t if t.is_contiguous() else t.contiguous()
+    return _dense(t)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent in builds of torch without a GPU runtime
@@ -719,6 +719,10 @@ def _as_rows(t: torch.Tensor):
     if t.stride(-1) == 1 and (t.dim() == 2 or (t.dim() == 3 and t.stride(0) == t.shape[1] * t.stride(1))):
         return t, t.stride(-2)
     return t.contiguous(), t.shape[-1]
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _as_btf(t: torch.Tensor):
@@ -753,8 +757,8 @@ def rms_norm_forward(x, residual, weight, eps: float, want_rstd: bool, quantize:
         _act(residual, "residual", x.shape, x)
         residual, ld_res = _as_rows(residual)
     rows = x.numel() // C
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    r = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    y = x.new_empty(x.shape)
+    r = x.new_empty(x.shape) if residual is not None else None
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
     q = e = None
     if quantize:
@@ -779,7 +783,7 @@ def rms_norm_backward(r, dy, dr, weight, rstd, want_dx: bool, want_dw: bool, win
     if dr is not None:
         dr, ld_dr = _as_rows(dr)
     dev = r.device
-    dx = torch.empty(r.shape, dtype=r.dtype, device=dev) if want_dx else None
+    dx = r.new_empty(r.shape) if want_dx else None
     if window is not None and (window.numel != C or window.base.shape[0] < groups):
         raise DpkError("rms_norm: grad-sample window does not match the layer")
     dw = torch.empty(C, dtype=torch.float32, device=dev) if want_dw and window is None else None
@@ -818,8 +822,8 @@ def causal_conv_forward(x, weight, bias, state, lengths, silu: bool, want_state:
     """Returns y [B,T,D] and the state behind each sequence [B,W-1,D] (or None)."""
     x, weight, bias, state, lengths, W = _conv_args(x, weight, bias, state, lengths)
     B, T, D = x.shape
-    y = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-    out = torch.empty(B, W - 1, D, dtype=x.dtype, device=x.device) if want_state else None
+    y = x.new_empty((B, T, D))
+    out = x.new_empty((B, W - 1, D)) if want_state else None
     if B:
         _call("dpk_causal_conv_forward", x.device, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _addr(bias),
               _addr(state), _addr(lengths), y.data_ptr(), _addr(out), B, T, D, W, int(silu), ACT_DTYPES[x.dtype])
@@ -828,18 +832,18 @@ def causal_conv_forward(x, weight, bias, state, lengths, silu: bool, want_state:
 
 def causal_conv_backward(x, weight, bias, state, lengths, silu: bool, dy, dstate_out, want_dstate: bool, want_par: bool,
                          windows=None, scale: float = 1.0, accumulate: bool = False):
-    """Returns dx, dstate (or None) and the parameters' gradients: (dw [D,W], db [D] or None) summed over the batch, or None
-    with `windows` = (weight window, bias window or None): then their rows receive the per-sample gradients."""
-    x, weight, bias, state, lengths, W = _conv_args(x, weight, bias, state, lengths)
+    """For operands that causal_conv_forward has taken (only dy and dstate_out are looked at again).  Returns dx, dstate (or None)
+    and the parameters' gradients: (dw [D,W], db [D] or None) summed over the batch, or None with `windows` = (weight window, bias
+    window or None): then their rows receive the per-sample gradients."""
     B, T, D = x.shape
-    _act(dy, "dy", x.shape, x)
-    dy = _as_btf(dy)
-    if dstate_out is not None:
-        _act(dstate_out, "dstate", (B, W - 1, D), x)
-        dstate_out = dstate_out.contiguous()
+    W = weight.shape[1]
+    x, weight, bias, state, lengths = _as_btf(x), _dense(weight), _dense(bias), _dense(state), _dense(lengths)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise DpkError("causal_conv: the gradient does not match the output")
+    dy, dstate_out = _as_btf(dy), _dense(dstate_out)
     dev = x.device
-    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-    dstate = torch.empty(B, W - 1, D, dtype=x.dtype, device=dev) if want_dstate else None
+    dx = x.new_empty((B, T, D))
+    dstate = x.new_empty((B, W - 1, D)) if want_dstate else None
     nb = 0 if bias is None else D
     grads = None
     if want_par and windows is None:
@@ -971,7 +975,7 @@ def selective_scan_forward(inp: ScanInputs, want_kept: bool, want_state: bool):
     b, t, d = u.shape
     n = inp.A_log.shape[1]
     lib = load()
-    out = torch.empty(b, t, d, dtype=u.dtype, device=u.device)
+    out = u.new_empty((b, t, d))
     hT = torch.empty(b, d, n, dtype=torch.float32, device=u.device) if want_state else None
     g = lib.dpk_selective_scan_group()
     kept = torch.empty(b, (t + g - 1) // g, lib.dpk_selective_scan_state_rows(n), d, dtype=torch.float32,
@@ -990,9 +994,9 @@ def selective_scan_backward(inp: ScanInputs, kept, dout, dhT, want_dh0: bool, wa
     b, t, d = u.shape
     n = inp.A_log.shape[1]
     dev = u.device
-    _act(dout, "dout", u.shape, u)
-    dout = dout if dout.stride(2) == 1 or d == 1 else dout.contiguous()
-    dhT = _par(dhT, "dstate", (b, d, n), dev)
+    if dout.shape != u.shape or dout.dtype != u.dtype:
+        raise DpkError("selective_scan: the gradient does not match the output")
+    dout, dhT = _as_btf(dout), _dense(dhT)
     new = u.new_empty
     du, ddelta, dB, dC = new(u.shape), new(u.shape), new((b, t, n)), new((b, t, n))
     dz = new(u.shape) if inp.z is not None else None
