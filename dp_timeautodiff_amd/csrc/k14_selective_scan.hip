@@ -11,12 +11,15 @@
 // channels, so every access of a wave is one run of memory); B_t and C_t are the same for all channels and are staged in LDS for
 // GROUP steps at a time.
 // The backward pass needs the states in reverse.  Undoing the recurrence would divide by decays near 0, so the forward pass
-// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16), and the backward pass recomputes a
-// group's states and decays into registers.  So that three waves a SIMD fit (with eight states
-// a lane the group spilled, and waited for its spills: 3311 us against 1887 for the plainest form), a channel's states lie on LS = N / 4 lanes there; what
-// a channel has once per step (softplus, gates, loads, stores) is dealt over those lanes by step, passed round by lane swaps.
-// Per state and step: forward one v_exp_f32 (quarter rate) and four plain instructions, backward one and thirteen, and the sums
-// over channels for dB and dC, which take a halving tree over the lanes (about five more).
+// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16), and the backward pass recomputes
+// a group's states and decays into registers.  A channel's states lie on LS = N / 4 lanes there, so that three waves a SIMD fit
+// (with all 16 on one lane, one wave a SIMD: 1887 us at 256 x 256 x 1024; with eight, the group spilled and waited for its spills:
+// 3311); what a channel has once per step (softplus, gates, loads, stores) is dealt over those lanes by step, and passed round by
+// lane swaps.
+// Per state and step: forward one v_exp_f32 (quarter rate) and four plain instructions, backward one and twelve, and the sums
+// over channels for dB and dC, a halving tree over the lanes (four more).  Measured at 256 x 256 x 1024, N = 16, fp32: forward
+// 360 us = 4.5 TB/s with the kept states, backward 950 us, bound by the vector ALU (about 80 % busy), of which 2.4 GB of traffic are
+// 500 us.
 // Sequences x channels / 64 is the number of waves; few long sequences are cut into chunks of time: each chunk's effect is
 // (decay, state from zero), which a short kernel joins in order, and the chunks then run side by side from their true states.
 #include "ssm_common.h"
@@ -357,9 +360,28 @@ __device__ __forceinline__ void fold_dpp(float* v) {
     }
 }
 constexpr int half_of(int c) { return c > 1 ? c / 2 : 1; }
-// V = 4 values over the 64 / LS low lanes
+// Four values over the 64 / LS low lanes.  At N = 16 (LS = 4) the halving is by DPP adds that write only the banks (four lanes) a value
+// stays on, which the compiler does not form from a choice and an add (11 instructions: 985 us at 256 x 256 x 1024, 950 so).  A
+// DPP operand may be read two wait states after its write: the s_nops, with the independent adds between them, keep that.
 template <int LS>
 __device__ __forceinline__ float lane_sums(float (&v)[4]) {
+    if constexpr (LS == 4) {
+        float a, b, r;
+        asm("s_nop 1\n\t"
+            "v_add_f32_dpp %0, %3, %3 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %1, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %0, %5, %5 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+            "v_add_f32_dpp %1, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+            "s_nop 0\n\t"
+            "v_add_f32_dpp %2, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %2, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+            "s_nop 1\n\t"
+            "v_add_f32_dpp %0, %2, %2 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+            "s_nop 1\n\t"
+            "v_add_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf"
+            : "=&v"(a), "=&v"(b), "=&v"(r) : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]));
+        return a;
+    }
     constexpr int C1 = LS == 1 ? 2 : 4, C2 = LS <= 2 ? half_of(C1) : 4, C3 = LS <= 4 ? half_of(C2) : 4;
     constexpr int C4 = half_of(C3), C5 = half_of(C4);
     if constexpr (LS == 1) fold32<4>(v);
