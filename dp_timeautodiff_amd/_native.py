@@ -672,6 +672,9 @@ ACT8_BLOCK = 128
 
 def _act(t, name: str, shape=None, like: Optional[torch.Tensor] = None):
     """An activation: HIP tensor of an activation dtype, of `shape`, with `like`'s dtype and device."""
+    if (like is not None and isinstance(t, torch.Tensor) and t.dtype is like.dtype and t.device == like.device
+            and (shape is None or t.shape == shape)):
+        return  # as `like`, which has been looked at
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise DpkError(f"{name}: expected a CUDA/HIP tensor (this package has no CPU path)")
     if t.dtype not in ACT_DTYPES:
@@ -686,6 +689,8 @@ def _par(t, name: str, shape, device, dtype=torch.float32):
     """A parameter, state or index vector: dense, of one shape, on the activations' device."""
     if t is None:
         return None
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape:
+        return _dense(t)
     _req(t, name, dtype)
     if tuple(t.shape) != tuple(shape) or t.device != device:
         raise DpkError(f"{name}: expected shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
@@ -726,8 +731,10 @@ def _dense(t):
 
 
 def _as_btf(t: torch.Tensor):
-    """[B, T, F] whose last dimension is contiguous."""
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+    """[B, T, F] whose last dimension is contiguous (and whose rows are less than 2^26 elements apart: the scan's lanes count a
+    group's rows in 32-bit byte offsets)."""
+    s = t.stride()
+    return t if (s[2] == 1 or t.shape[2] == 1) and s[1] < 1 << 26 else t.contiguous()
 
 
 def _sum_rows(device, src: int, groups: int, rows: int, in_stride: int, outs, scale: float, accumulate: bool):
@@ -928,7 +935,10 @@ class ScanInputs:
             _act(t, name, rows + (n,), u)
         if z is not None:
             _act(z, "z", u.shape, u)
-        dense = (lambda t: t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous())
+        if step:
+            dense = (lambda t: t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous())
+        else:
+            dense = (lambda t: None if t is None else _as_btf(t))
         self.u, self.delta, self.B, self.C, self.z = (dense(t) for t in (u, delta, B, C, z))
         dev = u.device
         self.A_log = _par(A_log, "A_log", (d, n), dev)

@@ -26,7 +26,7 @@ class Activation8(NamedTuple):
 
 def compress_activation(x: torch.Tensor) -> Activation8:
     """x [..., C] fp32, bf16 or fp16 on a HIP device."""
-    return Activation8(*_native.compress_activation(x.detach()), x.dtype)
+    return Activation8(*_native.compress_activation(x), x.dtype)
 
 
 def restore_activation(a: Activation8, dtype: torch.dtype = None) -> torch.Tensor:

@@ -249,7 +249,9 @@ class _Claim:
 
     @property
     def anchor(self):
-        return self._gsm._tap_on(self._layer.params[0].device)
+        # a leaf of its own for every call: one that an older graph still held would tie a captured backward pass to the
+        # stream of that graph
+        return torch.empty((), device=self._layer.params[0].device, requires_grad=True)
 
     @property
     def batch_first(self):
@@ -494,7 +496,9 @@ class GradSampleModule(nn.Module):
                 if isinstance(output, torch.Tensor) and not output.requires_grad:
                     # first layer of the model (its input is data): nothing upstream needs a gradient, but the
                     # backward hook must still see grad_output -> keep the output in the graph at zero cost
-                    tapped = _GradTap.apply(output, self._tap_on(output.device))
+                    if self._tap.device != output.device:
+                        object.__setattr__(self, "_tap", torch.zeros((), device=output.device, requires_grad=True))
+                    tapped = _GradTap.apply(output, self._tap)
             if not self.hooks_enabled or not module.training or not torch.is_grad_enabled():
                 return tapped
             if self.activation_bits == 8 and layer.kind == "linear":
@@ -527,11 +531,6 @@ class GradSampleModule(nn.Module):
                 self._materialise(layer)
 
         return hook
-
-    def _tap_on(self, device):
-        if self._tap.device != device:
-            object.__setattr__(self, "_tap", torch.zeros((), device=device, requires_grad=True))
-        return self._tap
 
     # ---- the deferred contraction ---------------------------------------------------------------------
     def _stack(self, tensors: List[torch.Tensor], feat_dims: int, batch_first: Optional[bool] = None) -> torch.Tensor:

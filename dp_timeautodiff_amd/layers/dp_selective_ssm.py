@@ -75,7 +75,7 @@ def causal_conv(x, weight, bias=None, *, activation: Optional[str] = "silu", sta
 
 def causal_conv_step(x, state, weight, bias=None, *, activation: Optional[str] = "silu"):
     """One token: x [B,D]; `state` [B,W-1,D] is updated in place.  Not differentiable."""
-    return _native.causal_conv_step(x.detach(), state, weight.detach(), None if bias is None else bias.detach(), _silu(activation))
+    return _native.causal_conv_step(x, state, weight, bias, _silu(activation))
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -125,8 +125,8 @@ def selective_scan(u, delta, A_log, B, C, D=None, z=None, dt_bias=None, *, softp
 
 def selective_scan_step(u, delta, A_log, B, C, state, D=None, z=None, dt_bias=None, *, softplus: bool = True):
     """One token: u, delta, z [B,D], B, C [B,N]; `state` [B,D,N] is updated in place.  Not differentiable."""
-    det = [None if t is None else t.detach() for t in (u, delta, A_log, B, C, D, z, dt_bias)]
-    return _native.selective_scan_step(_native.ScanInputs(*det, None, None, softplus, step=True), state)
+    return _native.selective_scan_step(_native.ScanInputs(u, delta, A_log, B, C, D, z, dt_bias, None, None, softplus, step=True),
+                                       state)
 
 
 class DPCausalConv(nn.Module):

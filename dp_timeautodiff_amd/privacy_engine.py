@@ -86,7 +86,7 @@ class PrivacyEngine:
         return data_loader
 
     def _prepare_model(self, module: nn.Module, *, batch_first: bool = True, loss_reduction: str = "mean",
-                       grad_sample_mode: str = "hooks") -> GradSampleModule:
+                       grad_sample_mode: str = "hooks", activation_bits: Optional[int] = None) -> GradSampleModule:
         self.validate(module=module, optimizer=None, data_loader=None)
         if grad_sample_mode not in ("hooks",):
             raise NotImplementedError(f"grad_sample_mode='{grad_sample_mode}': only 'hooks' is implemented")
@@ -96,13 +96,17 @@ class PrivacyEngine:
                                  f"Got: module.batch_first: {module.batch_first}, module.loss_reduction: "
                                  f"{module.loss_reduction}Requested: batch_first:{batch_first}, "
                                  f"loss_reduction: {loss_reduction}. Please pass vanilla nn.Module instead")
+            if activation_bits is not None and module.activation_bits != activation_bits:
+                raise ValueError(f"Pre-existing GradSampleModule has activation_bits={module.activation_bits}, requested: "
+                                 f"{activation_bits}. Please pass vanilla nn.Module instead")
             return module
         inner = module.module if isinstance(module, DPDDP) else module
         if self.fuse_recurrence and next(inner.parameters()).is_cuda:
             # CustomGRU-shaped loops -> the K8 recurrence kernels (same Linear submodules and parameters, so the
             # optimizer built on them stays valid)
             inner = fuse_recurrences(inner)
-        return GradSampleModule(inner, batch_first=batch_first, loss_reduction=loss_reduction)
+        return GradSampleModule(inner, batch_first=batch_first, loss_reduction=loss_reduction,
+                                activation_bits=32 if activation_bits is None else activation_bits)
 
     def is_compatible(self, *, module: nn.Module, optimizer: Optional[optim.Optimizer],
                       data_loader: Optional[DataLoader]) -> bool:
@@ -130,6 +134,7 @@ class PrivacyEngine:
             raise ValueError("Passing seed is prohibited in secure mode")
         self.fuse_recurrence = bool(kwargs.pop("fuse_recurrence", getattr(self, "fuse_recurrence", True)))
         device_sampler = bool(kwargs.pop("device_sampler", False))
+        activation_bits = kwargs.pop("activation_bits", None)  # 8: Linear inputs wait for the backward pass in 8 bits
 
         # compare module parameter with optimizer parameters
         model_parameters = set(module.parameters())
@@ -143,7 +148,7 @@ class PrivacyEngine:
                                       "not torch DDP: gradients are all-reduced by DistributedDPOptimizer")
 
         module = self._prepare_model(module, batch_first=batch_first, loss_reduction=loss_reduction,
-                                     grad_sample_mode=grad_sample_mode)
+                                     grad_sample_mode=grad_sample_mode, activation_bits=activation_bits)
         if poisson_sampling:
             module.forbid_grad_accumulation = True
 
@@ -180,7 +185,7 @@ class PrivacyEngine:
                           "Returned noise_multiplier assumes zero starting point, so your overall privacy "
                           "budget will be higher.")
         # options of this engine (not of the sigma search) travel on to make_private
-        engine_kw = {k: kwargs.pop(k) for k in ("device_sampler", "fuse_recurrence", "noise_seed") if k in kwargs}
+        engine_kw = {k: kwargs.pop(k) for k in ("device_sampler", "fuse_recurrence", "noise_seed", "activation_bits") if k in kwargs}
         return self.make_private(
             module=module, optimizer=optimizer, data_loader=data_loader,
             noise_multiplier=get_noise_multiplier(target_epsilon=target_epsilon, target_delta=target_delta,

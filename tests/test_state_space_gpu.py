@@ -203,7 +203,8 @@ SCAN = [  # B, T, D, N, options: z gate, d skip, b bias, s softplus, h state; le
     (1, 1, 1, 1, "zdbsh", None), (2, 7, 63, 4, "zdbs", None), (3, 8, 64, 16, "zdbsh", None), (2, 9, 65, 13, "zdbsh", [9, 3]),
     (4, 24, 250, 16, "zdbs", None), (3, 17, 300, 5, "sh", [17, 0, 8]), (2, 33, 520, 16, "zdbsh", [1, 33]), (2, 12, 70, 17, "zdbs", None),
     (2, 21, 40, 32, "zdbsh", [21, 16]), (2, 10, 30, 8, "dbh", None), (2, 0, 5, 4, "zdbsh", None), (0, 3, 5, 4, "zdbs", None),
-    (2, 1000, 70, 16, "zdbsh", [1000, 130]), (1, 650, 257, 4, "zds", None), (5, 5, 256, 16, "zdbs", None)]
+    (2, 1000, 70, 16, "zdbsh", [1000, 130]), (1, 650, 257, 4, "zds", None), (5, 5, 256, 16, "zdbs", None),
+    (1, 700, 40, 16, "sh", [611]), (1, 500, 20, 32, "zdbsh", None), (1, 9001, 3, 7, "zdbsh", None), (3, 300, 8, 8, "bs", [300, 0, 64])]
 
 
 def scan_inputs(case, dtype, seed=0):
@@ -419,7 +420,11 @@ def test_offsets_past_32_bits():
     assert torch.equal(selective_scan(u, delta, dense[2], dense[3], dense[4], dense[5], z, dense[7]), selective_scan(*dense[:8]))
     w = make(1, torch.float32, (D, 4))[0].cuda()
     assert torch.equal(causal_conv(u, w), causal_conv(dense[0], w))
-    del u, delta, z, buf
+    rows = buf.as_strided((2, T, D), (D, 2 ** 27, 1), 0)   # rows 2^27 elements apart
+    rows.copy_(dense[0])
+    assert torch.equal(selective_scan(rows, dense[1], dense[2], dense[3], dense[4]), selective_scan(*dense[:5]))
+    assert torch.equal(causal_conv(rows, w), causal_conv(dense[0], w))
+    del u, delta, z, rows, buf
     x = torch.empty(2 ** 24 + 3, 130, dtype=torch.bfloat16, device="cuda").fill_(1.5)  # 2.2e9 elements
     x[-1] = make(2, torch.bfloat16, (130,))[0].cuda()
     y, _ = rms_norm(x, torch.ones(130, device="cuda"))

@@ -131,6 +131,37 @@ def test_per_sample_gradients_and_the_optimizer_tail(dev, B, T, ragged):
     assert rel_err(got, ((flat * clip[:, None]).sum(0) / B).numpy()) < TOL
 
 
+@pytest.mark.parametrize("shared", [False, True])
+def test_per_sample_gradients_of_few_long_sequences(dev, shared):
+    """A sample's rows are spread over workgroups (norm, convolution) and chunks of time (scan), whose parts are joined; a layer's
+    second call adds to the joined rows."""
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    T = 300 if dev.type == "cuda" else 40
+    net = make_net(dev, shared=shared)
+    x, w = data(2, T)
+    lengths = torch.tensor([T, T - 27], dtype=torch.int32)
+    w = w * (torch.arange(T)[None, :, None] < lengths[:, None, None])
+    want = reference(net, x, w, lengths)
+    gsm = GradSampleModule(net, loss_reduction="sum")
+    (gsm(x.to(dev), lengths.to(dev)) * w.to(dev)).sum().backward()
+    gsm.check_complete()
+    check(net, want)
+
+
+def test_privacy_engine_hands_the_stash_width_on(dev):
+    from torch.utils.data import DataLoader, TensorDataset
+    from dp_timeautodiff_amd.privacy_engine import PrivacyEngine
+    net = make_net(dev)
+    loader = DataLoader(TensorDataset(torch.randn(16, 5, 5), torch.randn(16, 5, 3)), batch_size=8)
+    gsm, opt, _ = PrivacyEngine().make_private(module=net, optimizer=torch.optim.SGD(net.parameters(), lr=0.1), data_loader=loader,
+                                               noise_multiplier=1.0, max_grad_norm=1.0, poisson_sampling=False, activation_bits=8)
+    assert gsm.activation_bits == 8
+    x, w = data(4, 5)
+    (gsm(x.to(dev)) * w.to(dev)).mean().backward()
+    opt.step()
+    assert all(torch.isfinite(p).all() for p in net.parameters())
+
+
 def test_without_the_engine_the_layers_train_as_any_other(dev):
     net = make_net(dev)
     x, w = data(4, 7)
