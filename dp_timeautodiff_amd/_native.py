@@ -988,7 +988,7 @@ def selective_scan_forward(inp: ScanInputs, want_kept: bool, want_state: bool):
     out = u.new_empty((b, t, d))
     hT = torch.empty(b, d, n, dtype=torch.float32, device=u.device) if want_state else None
     g = lib.dpk_selective_scan_group()
-    kept = torch.empty(b, (t + g - 1) // g, lib.dpk_selective_scan_state_rows(n), d, dtype=torch.float32,
+    kept = torch.empty(b, max((t + g - 1) // g - (inp.h0 is None), 1), lib.dpk_selective_scan_state_rows(n), d, dtype=torch.float32,
                        device=u.device) if want_kept else None
     if b:
         s, scratch = inp.desc(kept)

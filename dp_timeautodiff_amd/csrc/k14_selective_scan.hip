@@ -11,14 +11,14 @@
 // channels, so every access of a wave is one run of memory); B_t and C_t are the same for all channels and are staged in LDS for
 // GROUP steps at a time.
 // The backward pass needs the states in reverse.  Undoing the recurrence would divide by decays near 0, so the forward pass
-// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16), and the backward pass recomputes
+// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16; not of the first group where it is 0), and the backward pass recomputes
 // a group's states and decays into registers.  A channel's states lie on LS = N / 4 lanes there, so that three waves a SIMD fit
 // (with all 16 on one lane, one wave a SIMD: 1887 us at 256 x 256 x 1024; with eight, the group spilled and waited for its spills:
 // 3311); what a channel has once per step (softplus, gates, loads, stores) is dealt over those lanes by step, and passed round by
 // lane swaps.
 // Per state and step: forward one v_exp_f32 (quarter rate) and four plain instructions, backward one and twelve, and the sums
 // over channels for dB and dC, a halving tree over the lanes (four more).  Measured at 256 x 256 x 1024, N = 16, fp32: forward
-// 360 us = 4.5 TB/s with the kept states, backward 950 us, bound by the vector ALU (about 80 % busy), of which 2.4 GB of traffic are
+// 350 us = 4.5 TB/s with the kept states, backward 955 us, bound by the vector ALU (about 80 % busy), of which 2.4 GB of traffic are
 // 500 us.
 // Sequences x channels / 64 is the number of waves; few long sequences are cut into chunks of time: each chunk's effect is
 // (decay, state from zero), which a short kernel joins in order, and the chunks then run side by side from their true states.
@@ -33,7 +33,7 @@ struct ScanArgs {
     const float *A_log, *Dskip, *dt_bias, *h0, *dhT;
     const int* lengths;
     void *out, *du, *ddelta, *dB, *dC, *dz;
-    float *hT, *dh0, *kept;     // kept: [b][group][n][d], n padded to 4, 8, 16 or 32
+    float *hT, *dh0, *kept;     // kept: [b][group][n][d], from step kept_from on, n padded to 4, 8, 16 or 32
     float *edge, *span;         // chunk edges: [chunk][b][n][d] and sums of dt [chunk][b][d]
     float *dbc;                 // [d block][b][t][2N] partial sums of dB | dC, where a row of channels needs several workgroups
     float *dA, *dD, *dbias;     // parameter gradients, row (b * nchunk + chunk) of par_stride floats
@@ -130,6 +130,36 @@ __device__ __forceinline__ float elem(const void* p, int64_t sb, int64_t st, int
 
 __device__ __forceinline__ float step_size(const ScanArgs& a, float pre) { return a.softplus ? softplus_f(pre).value : pre; }
 
+// first step whose state the forward pass keeps: without h0 the first group's is 0
+__device__ __forceinline__ int kept_from(const ScanArgs& a) { return a.h0 ? 0 : GROUP; }
+
+// N numbers of a channel, which lie together: four at a time
+template <int NT>
+__device__ __forceinline__ void load_states(const float* __restrict__ p, int n, float (&v)[NT]) {
+#pragma unroll
+    for (int k = 0; k < NT; k += 4) {
+        float t[4];
+        load_n<float, 4>(p + k, n - k, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[k + i] = t[i];
+    }
+}
+template <int NT>
+__device__ __forceinline__ void store_states(float* __restrict__ p, int n, const float (&v)[NT]) {
+#pragma unroll
+    for (int k = 0; k < NT; k += 4) {
+        const float t[4] = {v[k], v[k + 1], v[k + 2], v[k + 3]};
+        store_n<float, 4>(p + k, n - k, t);
+    }
+}
+// -exp(A_log) log2 e of states n0 ..., 0 behind N
+template <int NT>
+__device__ __forceinline__ void decay_rates(const ScanArgs& a, int d, int n0, float (&A2)[NT]) {
+    load_states<NT>(a.A_log + (int64_t)d * a.N + n0, a.N - n0, A2);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) A2[n] = n0 + n < a.N ? -expf(A2[n]) * LOG2E : 0.f;
+}
+
 // EDGE: only the chunk's state from zero and its sum of dt, for the chunks' joining
 template <typename T, int NT, bool EDGE>
 __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_forward_kernel(ScanArgs a) {
@@ -138,26 +168,25 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_forward_kernel(Sca
     const int end = seq_end(a, p.b);
     const int dd = p.live ? p.d : a.D - 1;   // lanes behind the last channel read it and store nothing
     float A2[NT], h[NT];
+    decay_rates<NT>(a, dd, 0, A2);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        A2[n] = n < a.N ? -expf(a.A_log[(int64_t)dd * a.N + n]) * LOG2E : 0.f;
-        h[n] = 0.f;
-        if (!EDGE && n < a.N) {
-            if (a.nchunk > 1)
-                h[n] = a.edge[(((int64_t)p.chunk * a.nb + p.b) * a.N + n) * a.D + dd];
-            else if (a.h0)
-                h[n] = a.h0[((int64_t)p.b * a.D + dd) * a.N + n];
-        }
+    for (int n = 0; n < NT; ++n) h[n] = 0.f;
+    if (!EDGE && a.nchunk > 1) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            if (n < a.N) h[n] = a.edge[(((int64_t)p.chunk * a.nb + p.b) * a.N + n) * a.D + dd];
+    } else if (!EDGE && a.h0) {
+        load_states<NT>(a.h0 + ((int64_t)p.b * a.D + dd) * a.N, a.N, h);
     }
     const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f;
     const float skip = a.Dskip ? a.Dskip[dd] : 0.f;
     float span = 0.f;
-    const int ngroup = (a.T + GROUP - 1) / GROUP;
+    const int k0 = kept_from(a), ngroup = (a.T - k0 + GROUP - 1) / GROUP;   // groups with a kept state
     const uint32_t lane_in = (uint32_t)dd * sizeof(T), lane_out = (uint32_t)p.d * sizeof(T);
     int ph = 0;
     for (int t0 = p.t0; t0 < p.t1; t0 += GROUP, ph ^= 1) {
-        if (!EDGE && a.kept && p.live) {
-            char* k = (char*)(a.kept + ((int64_t)p.b * ngroup + t0 / GROUP) * NT * a.D);
+        if (!EDGE && a.kept && p.live && t0 >= k0) {
+            char* k = (char*)(a.kept + ((int64_t)p.b * ngroup + (t0 - k0) / GROUP) * NT * a.D);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 if (n < a.N) put<float>(k + (int64_t)n * a.D * 4, (uint32_t)p.d * 4u, h[n]);
@@ -211,9 +240,7 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_forward_kernel(Sca
             if (n < a.N) a.edge[(((int64_t)p.chunk * a.nb + p.b) * a.N + n) * a.D + p.d] = h[n];
         a.span[((int64_t)p.chunk * a.nb + p.b) * a.D + p.d] = span;
     } else if (a.hT && p.chunk == a.nchunk - 1) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (n < a.N) a.hT[((int64_t)p.b * a.D + p.d) * a.N + n] = h[n];
+        store_states<NT>(a.hT + ((int64_t)p.b * a.D + p.d) * a.N, a.N, h);
     }
 }
 
@@ -284,11 +311,9 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_backward_edge_kern
     const int end = seq_end(a, p.b);
     const int dd = p.live ? p.d : a.D - 1;
     float A2[NT], dh[NT];
+    decay_rates<NT>(a, dd, 0, A2);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        A2[n] = n < a.N ? -expf(a.A_log[(int64_t)dd * a.N + n]) * LOG2E : 0.f;
-        dh[n] = 0.f;
-    }
+    for (int n = 0; n < NT; ++n) dh[n] = 0.f;
     const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f;
     const uint32_t lane_in = (uint32_t)dd * sizeof(T);
     float span = 0.f;
@@ -470,25 +495,27 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
     const bool live = d < a.D;
     const int dd = live ? d : a.D - 1;
     const int lo = chunk * a.chunk, hi = lo + a.chunk < a.T ? lo + a.chunk : a.T;
-    const int end = seq_end(a, b);
     float A2[S], dh[S], dA[S];
+    decay_rates<S>(a, dd, n0, A2);
 #pragma unroll
-    for (int j = 0; j < S; ++j) {
-        const int n = n0 + j;
-        A2[j] = n < a.N ? -expf(a.A_log[(int64_t)dd * a.N + n]) * LOG2E : 0.f;
-        dA[j] = 0.f;
-        dh[j] = 0.f;
-        if (n < a.N && live) {   // lanes behind the last channel stay 0: nothing of them may reach the sums over channels
-            if (a.nchunk > 1)
-                dh[j] = a.edge[(((int64_t)chunk * a.nb + b) * a.N + n) * a.D + dd];
-            else if (a.dhT)
-                dh[j] = a.dhT[((int64_t)b * a.D + dd) * a.N + n];
-        }
-    }
+    for (int j = 0; j < S; ++j) dA[j] = 0.f;
     const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f;
     const float skip = a.Dskip ? a.Dskip[dd] : 0.f;
     float dD = 0.f, dbias = 0.f;
-    const int ngroup = (a.T + GROUP - 1) / GROUP;
+    const int k0 = kept_from(a), ngroup = (a.T - k0 + GROUP - 1) / GROUP;   // groups with a kept state
+    int ph = 0;
+    const int end = seq_end(a, b);
+#pragma unroll
+    for (int j = 0; j < S; ++j) dh[j] = 0.f;
+    if (live) {   // lanes behind the last channel stay 0: nothing of them may reach the sums over channels
+        if (a.nchunk > 1) {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (n0 + j < a.N) dh[j] = a.edge[(((int64_t)chunk * a.nb + b) * a.N + n0 + j) * a.D + dd];
+        } else if (a.dhT) {
+            load_states<S>(a.dhT + ((int64_t)b * a.D + dd) * a.N + n0, a.N - n0, dh);
+        }
+    }
     // The group being fetched, as it lies in memory.  Steps behind the sequence read the group's first row instead and count as
     // zeros where the group is taken up, as do lanes behind the last channel.  (Not here: a choice right behind a load becomes a
     // branch round it and a wait for it, in the middle of the arithmetic that is to hide it.)
@@ -512,7 +539,7 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
             ndy[i] = at<T>(go, (r * (uint32_t)a.dout_st + dd) * (uint32_t)sizeof(T));
             nz[i] = at<T>(gz, (r * (uint32_t)a.z_st + dd) * (uint32_t)sizeof(T));
         }
-        const char* k = (const char*)(a.kept + ((int64_t)b * ngroup + t0 / GROUP) * NT * a.D);
+        const char* k = (const char*)(a.kept + ((int64_t)b * ngroup + (t0 > k0 ? (t0 - k0) / GROUP : 0)) * NT * a.D);
 #pragma unroll
         for (int j = 0; j < S; ++j) nh[j] = at<float>(k, lane_kept + (uint32_t)j * (uint32_t)a.D * 4u);
     };
@@ -530,20 +557,19 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
         for (int i = threadIdx.x; i < GROUP * 2 * a.N; i += blockDim.x) {
             const int q = i / (2 * a.N), r = i % (2 * a.N);
             if (t0 + q >= hi) continue;
-            const int64_t row = (int64_t)b * a.T + t0 + q;
+            const int64_t bt = (int64_t)b * a.T + t0 + q;
             if (a.ndb > 1)
-                a.dbc[((int64_t)dblk * a.nb * a.T + row) * 2 * a.N + r] = 0.f;
+                a.dbc[((int64_t)dblk * a.nb * a.T + bt) * 2 * a.N + r] = 0.f;
             else if (r < a.N)
-                ((T*)a.dB)[row * a.N + r] = (T)0.f;
+                ((T*)a.dB)[bt * a.N + r] = (T)0.f;
             else
-                ((T*)a.dC)[row * a.N + r - a.N] = (T)0.f;
+                ((T*)a.dC)[bt * a.N + r - a.N] = (T)0.f;
         }
     }
-    int ph = 0;
     if (t0 >= lo) {
         fetch(t0);
         fetch_bc<T, NT>(a, b, t0, end, nbc);
-        put_bc<T, NT>(a, b, t0, end, nbc, bc[0]);
+        put_bc<T, NT>(a, b, t0, end, nbc, bc[ph]);
         __syncthreads();
     }
     for (; t0 >= lo; t0 -= GROUP) {
@@ -554,6 +580,7 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
         uint32_t to = lane_out;
         asm volatile("" : "+v"(to));
         fetch_bc<T, NT>(a, b, next, end, nbc);
+        {
         {
             float xs[OWN];
 #pragma unroll
@@ -578,7 +605,7 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
         {
             float h[S];
 #pragma unroll
-            for (int j = 0; j < S; ++j) h[j] = n0 + j < a.N && live ? nh[j] : 0.f;
+            for (int j = 0; j < S; ++j) h[j] = n0 + j < a.N && live && t0 >= k0 ? nh[j] : 0.f;
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -650,6 +677,7 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
                 put<T>((char*)a.ddelta + o, to, in ? dpre : 0.f);
             }
         }
+        }
         __syncthreads();   // the group's sums are written, the next group's B and C staged
         for (int i = threadIdx.x; i < GROUP * 2 * NT; i += blockDim.x) {
             const int q = i / (2 * NT), r = i % (2 * NT), n = r % NT;
@@ -657,21 +685,17 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
             float s = 0.f;
             if (t0 + q < end)
                 for (int w = 0; w < nw; ++w) s += part[ph][w][q][r];
-            const int64_t row = (int64_t)b * a.T + t0 + q;
+            const int64_t bt = (int64_t)b * a.T + t0 + q;
             if (a.ndb > 1)
-                a.dbc[((int64_t)dblk * a.nb * a.T + row) * 2 * a.N + (r < NT ? n : a.N + n)] = s;
+                a.dbc[((int64_t)dblk * a.nb * a.T + bt) * 2 * a.N + (r < NT ? n : a.N + n)] = s;
             else if (r < NT)
-                ((T*)a.dB)[row * a.N + n] = (T)s;
+                ((T*)a.dB)[bt * a.N + n] = (T)s;
             else
-                ((T*)a.dC)[row * a.N + n] = (T)s;
+                ((T*)a.dC)[bt * a.N + n] = (T)s;
         }
         ph ^= 1;
     }
-    if (a.dh0 && chunk == 0 && live) {
-#pragma unroll
-        for (int j = 0; j < S; ++j)
-            if (n0 + j < a.N) a.dh0[((int64_t)b * a.D + d) * a.N + n0 + j] = dh[j];
-    }
+    if (a.dh0 && chunk == 0 && live) store_states<S>(a.dh0 + ((int64_t)b * a.D + d) * a.N + n0, a.N - n0, dh);
     // dD and dbias are spread over the channel's lanes by step
 #pragma unroll
     for (int off = CPW; off < 64; off <<= 1) {
@@ -679,16 +703,20 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
         dbias += __shfl_xor(dbias, off, 64);
     }
     if (!live) return;
-    const int64_t row = ((int64_t)b * a.nchunk + chunk) * a.par_stride;
-    if (a.dA) {
-        float* o = a.dA + row + (int64_t)d * a.N + n0;
+    const int64_t at = ((int64_t)b * a.nchunk + chunk) * a.par_stride;
+    if (a.dA && n0 < a.N) {
+        float* o = a.dA + at + (int64_t)d * a.N + n0;
+        float old[S];
 #pragma unroll
-        for (int j = 0; j < S; ++j)
-            if (n0 + j < a.N) o[j] = (a.accumulate ? o[j] : 0.f) + a.scale * (A2[j] * LN2) * dA[j];
+        for (int j = 0; j < S; ++j) old[j] = 0.f;
+        if (a.accumulate) load_states<S>(o, a.N - n0, old);
+#pragma unroll
+        for (int j = 0; j < S; ++j) dA[j] = old[j] + a.scale * (A2[j] * LN2) * dA[j];
+        store_states<S>(o, a.N - n0, dA);
     }
     if (sb > 0) return;
-    if (a.dD) a.dD[row + d] = (a.accumulate ? a.dD[row + d] : 0.f) + a.scale * dD;
-    if (a.dbias) a.dbias[row + d] = (a.accumulate ? a.dbias[row + d] : 0.f) + a.scale * dbias;
+    if (a.dD) a.dD[at + d] = (a.accumulate ? a.dD[at + d] : 0.f) + a.scale * dD;
+    if (a.dbias) a.dbias[at + d] = (a.accumulate ? a.dbias[at + d] : 0.f) + a.scale * dbias;
 }
 
 // dB and dC of all channel blocks, in their order

@@ -204,7 +204,8 @@ SCAN = [  # B, T, D, N, options: z gate, d skip, b bias, s softplus, h state; le
     (4, 24, 250, 16, "zdbs", None), (3, 17, 300, 5, "sh", [17, 0, 8]), (2, 33, 520, 16, "zdbsh", [1, 33]), (2, 12, 70, 17, "zdbs", None),
     (2, 21, 40, 32, "zdbsh", [21, 16]), (2, 10, 30, 8, "dbh", None), (2, 0, 5, 4, "zdbsh", None), (0, 3, 5, 4, "zdbs", None),
     (2, 1000, 70, 16, "zdbsh", [1000, 130]), (1, 650, 257, 4, "zds", None), (5, 5, 256, 16, "zdbs", None),
-    (1, 700, 40, 16, "sh", [611]), (1, 500, 20, 32, "zdbsh", None), (1, 9001, 3, 7, "zdbsh", None), (3, 300, 8, 8, "bs", [300, 0, 64])]
+    (1, 700, 40, 16, "sh", [611]), (1, 500, 20, 32, "zdbsh", None), (1, 9001, 3, 7, "zdbsh", None), (3, 300, 8, 8, "bs", [300, 0, 64]),
+    (700, 3, 240, 16, "zdbsh", None), (901, 9, 300, 4, "zdbs", [9, 0, 5] * 300 + [2])]
 
 
 def scan_inputs(case, dtype, seed=0):
