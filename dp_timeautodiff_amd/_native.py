@@ -63,8 +63,8 @@ EXPORTS = {
     "dpk_rms_norm_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_int64, c_int, c_float, c_int, c_void_p]),
     "dpk_rms_norm_split": (c_int, [c_int64, c_int64]),
-    "dpk_rms_norm_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
-                                      c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]),
+    "dpk_rms_norm_backward": (c_int, [c_void_p, c_int64] * 4 + [c_void_p] * 4
+                              + [c_int64] * 3 + [c_int, c_int, c_float, c_int, c_int, c_void_p]),
     "dpk_causal_conv_segments": (c_int, [c_int, c_int, c_int]),
     "dpk_causal_conv_forward": (c_int, [c_void_p, c_int64, c_int64] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
     "dpk_causal_conv_backward": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 8
@@ -777,16 +777,18 @@ def rms_norm_forward(x, residual, weight, eps: float, want_rstd: bool, quantize:
     return y, r, rstd, q, e
 
 
-def rms_norm_backward(r, dy, dr, weight, rstd, want_dx: bool, want_dw: bool, window: Optional[FlatView] = None,
+def rms_norm_backward(r, residual, dy, dr, weight, rstd, want_dx: bool, want_dw: bool, window: Optional[FlatView] = None,
                       scale: float = 1.0, accumulate: bool = False):
-    """r, dy, dr (None = zeros) [..., C].  Returns dx (or None) and the weight's gradient: [C] summed over all rows, or None with
+    """r, residual (None: r is the sum), dy, dr (None = zeros) [..., C].  Returns dx (or None) and the weight's gradient: [C] summed over all rows, or None with
     `window` given: then row b of the window receives (or is added) `scale` times the gradient of sample b = r[b]."""
     C = r.shape[-1]
     rows = r.numel() // C
     groups = r.shape[0] if window is not None else 1
     r, ld_r = _as_rows(r)
     dy, ld_dy = _as_rows(dy)
-    ld_dr = 0
+    ld_dr = ld_res = 0
+    if residual is not None:
+        residual, ld_res = _as_rows(residual)
     if dr is not None:
         dr, ld_dr = _as_rows(dr)
     dev = r.device
@@ -800,8 +802,8 @@ def rms_norm_backward(r, dy, dr, weight, rstd, want_dx: bool, want_dw: bool, win
     split = load().dpk_rms_norm_split(groups, per)
     out, stride = (None, C) if not want_dw else (window.ptr.value, window.stride) if window is not None else (dw.data_ptr(), C)
     ws = torch.empty(groups * split, C, dtype=torch.float32, device=dev) if split > 1 and want_dw else None
-    _call("dpk_rms_norm_backward", dev, r.data_ptr(), ld_r, dy.data_ptr(), ld_dy, _addr(dr), ld_dr, weight.data_ptr(),
-          rstd.data_ptr(), _addr(dx), out if ws is None else ws.data_ptr(), stride if ws is None else C, groups, per, split, C,
+    _call("dpk_rms_norm_backward", dev, r.data_ptr(), ld_r, _addr(residual), ld_res, dy.data_ptr(), ld_dy, _addr(dr), ld_dr,
+          weight.data_ptr(), rstd.data_ptr(), _addr(dx), out if ws is None else ws.data_ptr(), stride if ws is None else C, groups, per, split, C,
           scale if ws is None else 1.0, int(accumulate and ws is None), ACT_DTYPES[r.dtype])
     if ws is not None:
         _sum_rows(dev, ws.data_ptr(), groups, split, C, [(out, C, stride)], scale, accumulate)

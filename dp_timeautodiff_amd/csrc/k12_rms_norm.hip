@@ -5,7 +5,9 @@
 //   dw[c] = sum over a group's rows of dy * xhat (a group is one sample under DP-SGD, or all rows)
 //
 // HBM-bound: forward reads x and residual and writes y and r, backward reads r, dy, dr_out and writes dx; every element is touched
-// once, in registers, and the sums over a row and over a group's rows are fp32.  LPR lanes hold one row, E elements each, as
+// once, in registers, and the sums over a row and over a group's rows are fp32.  In 16 bits backward reads x and residual in place
+// of r: a weight gradient in fp32 from the rounded r would be off by up to half a step of r's type (1024 x 256 x 512 bf16: 260 us
+// against 213, five arrays in place of four).  Four waves a SIMD are held to: 65536 x 1000 fp16 takes 210 us with three, 161 so.  LPR lanes hold one row, E elements each, as
 // E / V accesses of 16 bytes; the norm is taken of the fp32 sum, before r is rounded to its type.
 #include "ssm_common.h"
 
@@ -122,12 +124,13 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256)
 }
 
 // One workgroup walks the rows of (group, split); its row slots keep their share of dw in registers and meet in LDS at the end.
-template <typename T, int E, int LPR>
-__global__ void __launch_bounds__(LPR > 256 ? LPR : 256)
-    rms_backward_kernel(const T* __restrict__ R, int64_t ld_r, const T* __restrict__ DY, int64_t ld_dy,
-                        const T* __restrict__ DR, int64_t ld_dr, const float* __restrict__ Wt,
-                        const float* __restrict__ RSTD, T* __restrict__ DX, float* __restrict__ DW, int64_t dw_stride,
-                        int64_t rows_per_group, int split, int C, float scale, int accumulate) {
+// SUM: r is R + RES.  HAS_DR: DR is added to DX.  (Compiled in: a branch round a load is waited for before the next load.)
+template <typename T, int E, int LPR, bool SUM, bool HAS_DR>
+__global__ void __launch_bounds__(LPR > 256 ? LPR : 256, 4)
+    rms_backward_kernel(const T* __restrict__ R, int64_t ld_r, const T* __restrict__ RES, int64_t ld_res,
+                        const T* __restrict__ DY, int64_t ld_dy, const T* __restrict__ DR, int64_t ld_dr,
+                        const float* __restrict__ Wt, const float* __restrict__ RSTD, T* __restrict__ DX, float* __restrict__ DW,
+                        int64_t dw_stride, int64_t rows_per_group, int split, int C, float scale, int accumulate) {
     constexpr int V = Vec<T>::N, K = E / V;
     constexpr int NT = LPR > 256 ? LPR : 256, RPB = NT / LPR;
     __shared__ float red[32];
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256)
     // two rows of a slot are under way where they fit the registers: 16 bytes a lane and row are too few to fill HBM's latency
     constexpr int NR = E <= 8 ? 2 : 1;
     for (int64_t r0 = lo; r0 < hi; r0 += RPB * NR) {
-        float x[NR][K][V], g[NR][K][V], d[NR][K][V], rstd[NR], dot[NR];
+        float x[NR][K][V], s[NR][K][V], g[NR][K][V], d[NR][K][V], rstd[NR], dot[NR];
         bool live[NR];
         int64_t row[NR];
 #pragma unroll
@@ -161,8 +164,9 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256)
                 const int c = (k * LPR + lane) * V;
                 const int n = live[j] && c < C ? C - c : 0;
                 load_n<T, V>(R + row[j] * ld_r + c, n, x[j][k]);
+                if (SUM) load_n<T, V>(RES + row[j] * ld_res + c, n, s[j][k]);
                 load_n<T, V>(DY + row[j] * ld_dy + c, n, g[j][k]);
-                if (DX && DR) load_n<T, V>(DR + row[j] * ld_dr + c, n, d[j][k]);
+                if (HAS_DR) load_n<T, V>(DR + row[j] * ld_dr + c, n, d[j][k]);
             }
         }
 #pragma unroll
@@ -171,6 +175,7 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256)
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
+                    if (SUM) x[j][k][i] += s[j][k][i];
                     x[j][k][i] *= rstd[j];
                     dw[k][i] += g[j][k][i] * x[j][k][i];
                     g[j][k][i] *= w[k][i];
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         o[i] = rstd[j] * (g[j][k][i] - x[j][k][i] * dot[j]);
-                        if (DR) o[i] += d[j][k][i];
+                        if (HAS_DR) o[i] += d[j][k][i];
                     }
                     store_n<T, V>(DX + row[j] * C + c, n, o);
                 }
@@ -265,20 +270,32 @@ extern "C" int dpk_rms_norm_split(int64_t groups, int64_t rows_per_group) {
     return (int)(s < 1 ? 1 : s);
 }
 
-extern "C" int dpk_rms_norm_backward(const void* R, int64_t ld_r, const void* DY, int64_t ld_dy, const void* DR, int64_t ld_dr,
-                                     const float* W, const float* rstd, void* DX, float* DW, int64_t dw_stride, int64_t groups,
-                                     int64_t rows_per_group, int split, int C, float scale, int accumulate, int dtype,
-                                     void* stream) {
-    if (groups < 0 || rows_per_group < 0 || split <= 0 || C <= 0 || ld_r < 0 || ld_dy < 0 || ld_dr < 0) return DPK_EINVAL;
-    if (DW && dw_stride < C) return DPK_EINVAL;
+extern "C" int dpk_rms_norm_backward(const void* R, int64_t ld_r, const void* RES, int64_t ld_res, const void* DY,
+                                     int64_t ld_dy, const void* DR, int64_t ld_dr, const float* W, const float* rstd, void* DX,
+                                     float* DW, int64_t dw_stride, int64_t groups, int64_t rows_per_group, int split, int C,
+                                     float scale, int accumulate, int dtype, void* stream) {
+    if (groups < 0 || rows_per_group < 0 || split <= 0 || C <= 0 || ld_r < 0 || ld_res < 0 || ld_dy < 0 || ld_dr < 0)
+        return DPK_EINVAL;
+    if ((DW && dw_stride < C) || (RES && dtype == DPK_F32)) return DPK_EINVAL;
     if (groups == 0) return DPK_OK;
     if (!W || (rows_per_group > 0 && (!R || !DY || !rstd))) return DPK_EINVAL;
     if (C > MAX_C || groups * split > 0x7fffffffLL) return DPK_ERANGE;
-#define RMS_CALL(T, E, LPR)                                                                                                      \
-    hipLaunchKernelGGL((rms_backward_kernel<T, E, LPR>), dim3((unsigned)(groups * split)), dim3(LPR > 256 ? LPR : 256), 0,     \
-                       (hipStream_t)stream, (const T*)R, ld_r, (const T*)DY, ld_dy, (const T*)DR, ld_dr, W, rstd, (T*)DX, DW, \
-                       dw_stride, rows_per_group, split, C, scale, accumulate)
+#define RMS_GO(T, E, LPR, SUM, HAS_DR)                                                                                           \
+    hipLaunchKernelGGL((rms_backward_kernel<T, E, LPR, SUM, HAS_DR>), dim3((unsigned)(groups * split)),                        \
+                       dim3(LPR > 256 ? LPR : 256), 0, (hipStream_t)stream, (const T*)R, ld_r, (const T*)RES, ld_res,           \
+                       (const T*)DY, ld_dy, (const T*)DR, ld_dr, W, rstd, (T*)DX, DW, dw_stride, rows_per_group, split, C, scale, \
+                       accumulate)
+#define RMS_CALL(T, E, LPR)                                    \
+    if (RES && DX && DR)                                       \
+        RMS_GO(T, E, LPR, (sizeof(T) == 2), true);             \
+    else if (RES)                                              \
+        RMS_GO(T, E, LPR, (sizeof(T) == 2), false);            \
+    else if (DX && DR)                                         \
+        RMS_GO(T, E, LPR, false, true);                        \
+    else                                                       \
+        RMS_GO(T, E, LPR, false, false)
     DPK_DISPATCH_DTYPE(dtype, T, RMS_PICK(T, C, RMS_CALL);)
 #undef RMS_CALL
+#undef RMS_GO
     return dpk_launch_status();
 }

@@ -24,7 +24,9 @@ class _RMSNorm(torch.autograd.Function):
         y, r, rstd, q, e = _native.rms_norm_forward(x, residual, weight, eps, True, quantize)
         ctx.set_materialize_grads(False)
         ctx.sink, ctx.has_residual = sink, residual is not None
-        ctx.save_for_backward(x if r is None else r, weight, rstd)
+        # in 16 bits r is rounded: the weight's gradient, which is not, goes by the sum itself
+        parts = (x, residual) if r is None or r.dtype != torch.float32 else (r, None)
+        ctx.save_for_backward(*parts, weight, rstd)
         out = (y,) if r is None else (y, r)
         if quantize:
             ctx.mark_non_differentiable(q, e)
@@ -34,7 +36,7 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dr=None, *_):
-        r, weight, rstd = ctx.saved_tensors
+        r, residual, weight, rstd = ctx.saved_tensors
         if not ctx.has_residual:
             dr = None
         need_x, need_res, need_w = ctx.needs_input_grad[:3]
@@ -42,11 +44,11 @@ class _RMSNorm(torch.autograd.Function):
             dy = torch.zeros_like(r)
         if ctx.sink is not None:
             with ctx.sink(r.shape[0]) as to:
-                dx, _ = _native.rms_norm_backward(r, dy, dr, weight, rstd, need_x or need_res, True, to.window("weight"), to.scale,
-                                                  to.accumulate)
+                dx, _ = _native.rms_norm_backward(r, residual, dy, dr, weight, rstd, need_x or need_res, True, to.window("weight"),
+                                                  to.scale, to.accumulate)
             dw = None
         else:
-            dx, dw = _native.rms_norm_backward(r, dy, dr, weight, rstd, need_x or need_res, need_w)
+            dx, dw = _native.rms_norm_backward(r, residual, dy, dr, weight, rstd, need_x or need_res, need_w)
         return dx if need_x else None, dx if need_res else None, dw, None, None, None, None
 
 

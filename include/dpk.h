@@ -338,16 +338,17 @@ int dpk_adam_step(const float* grad, float* exp_avg, float* exp_avg_sq, const in
  * K12: r = X + RES (RES NULL: r = X and R is not needed), rstd = 1/sqrt(mean_c r^2 + eps), Y = r * rstd * W over rows of C <=
  * 16384 elements.  R, rstd (rows floats) may be NULL.  Q [rows, C] and QE [rows, ceil(C/128)] (both or neither) receive Y in 8 bits, as
  * dpk_compress_activation would hold it.
- * backward: DX (nullable) = rstd * (g - xhat * mean_c(g * xhat)) + DR (nullable), g = DY * W, xhat = R * rstd.  The rows are `groups`
- * groups of rows_per_group; DW (nullable) row (group * split + k) receives scale * sum of DY * xhat over the k-th of `split` parts of
+ * backward: DX (nullable) = rstd * (g - xhat * mean_c(g * xhat)) + DR (nullable), g = DY * W, xhat = (R + RES) * rstd: R and RES are
+ * forward's X and RES in 16 bits (where its R is the rounded sum), or R and NULL.  The rows are `groups` groups of rows_per_group; DW (nullable) row (group * split + k) receives scale * sum of DY * xhat over the k-th of `split` parts of
  * the group's rows (accumulate: is added to).  dpk_rms_norm_split says how many parts fill the chip; dpk_sum_rows joins them.
  */
 int dpk_rms_norm_forward(const void* X, int64_t ld_x, const void* RES, int64_t ld_res, const float* W, void* Y, void* R,
                          float* rstd, int8_t* Q, uint8_t* QE, int64_t rows, int C, float eps, int dtype, void* stream);
 int dpk_rms_norm_split(int64_t groups, int64_t rows_per_group);
-int dpk_rms_norm_backward(const void* R, int64_t ld_r, const void* DY, int64_t ld_dy, const void* DR, int64_t ld_dr,
-                          const float* W, const float* rstd, void* DX, float* DW, int64_t dw_stride, int64_t groups,
-                          int64_t rows_per_group, int split, int C, float scale, int accumulate, int dtype, void* stream);
+int dpk_rms_norm_backward(const void* R, int64_t ld_r, const void* RES, int64_t ld_res, const void* DY, int64_t ld_dy,
+                          const void* DR, int64_t ld_dr, const float* W, const float* rstd, void* DX, float* DW,
+                          int64_t dw_stride, int64_t groups, int64_t rows_per_group, int split, int C, float scale,
+                          int accumulate, int dtype, void* stream);
 
 /*
  * K13: p_t = bias + sum_i w[d,i] x_{t-W+1+i}, y = p or silu(p), W <= 4, w [D,W], bias [D] or NULL.  x [B,T,D] with strides; rows

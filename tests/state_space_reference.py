@@ -100,8 +100,8 @@ def _per_sample(fn, B, *grads_of):
     return [torch.stack(g) for g in zip(*(fn(b) for b in range(B)))]
 
 
-def _rms_norm_backward(r, dy, dr, weight, rstd, want_dx, want_dw, window=None, scale=1.0, accumulate=False):
-    r64, s = r.double(), rstd.double().view(*r.shape[:-1], 1)
+def _rms_norm_backward(r, residual, dy, dr, weight, rstd, want_dx, want_dw, window=None, scale=1.0, accumulate=False):
+    r64, s = r.double() + (0 if residual is None else residual.double()), rstd.double().view(*r.shape[:-1], 1)
     n, g = r64 * s, dy.double() * weight.double()
     dx = s * (g - n * (g * n).mean(-1, keepdim=True)) + (0 if dr is None else dr.double())
     dw = dy.double() * n

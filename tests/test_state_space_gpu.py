@@ -73,21 +73,14 @@ def test_rms_norm(dtype, shape, residual):
     close(r, r_ref, "r")
     ((y_ref * dy.double()).sum() + (r_ref * dr.double()).sum()).backward()
     torch.autograd.backward((y, r), (dy.cuda(), dr.cuda()))
-    ex = ew = 0.0
-    if dtype != torch.float32 and residual and x.numel():
-        # backward reads r as stored: each r is off by eps / 2 of it, which moves xhat by as much
-        rr = r_ref.detach()
-        s = 1 / torch.sqrt((rr * rr).mean(-1, keepdim=True) + 1e-5)
-        n, g, h = rr * s, dy.double() * w.double(), torch.finfo(dtype).eps / 2
-        ex = h * s * n.abs() * ((g * n).mean(-1, keepdim=True).abs() + (g * n).abs().mean(-1, keepdim=True)) * 1.01
-        ew = h * (dy.double() * n).abs().reshape(-1, shape[-1]).sum(0) * 1.01
+    ex = 0.0
     if not residual and dtype != torch.float32:
         # r is x itself: autograd adds dr to the norm's already rounded gradient, so that one is rounded twice
         ex = torch.finfo(dtype).eps / 2 * (x64.grad - dr.double()).abs() * 1.01 + (2.0 ** -25 if dtype == torch.float16 else 0)
     close(xg.grad, x64.grad, "dx", ex)
     if residual:
         close(rg.grad, r64.grad, "dresidual", ex)
-    close(wg.grad, w64.grad, "dw", ew)
+    close(wg.grad, w64.grad, "dw")
 
 
 def test_rms_norm_reads_column_blocks_and_other_layouts():

@@ -369,8 +369,9 @@ def test_c_entry_refusals():
     assert norm(**ok(X=None)) == norm(**ok(W=None)) == norm(**ok(Y=None)) == norm(**ok(C=0)) == norm(**ok(rows=-1)) == -1
     assert norm(**ok(eps=-1.0)) == norm(**ok(eps=float("nan"))) == norm(**ok(dtype=3)) == norm(**ok(Q=p)) == norm(**ok(E=p)) == -1
     assert norm(**ok(C=16385)) == norm(**ok(rows=2 ** 31)) == -2
-    assert lib.dpk_rms_norm_backward(p, 8, p, 8, None, 0, p, p, p, p, 7, 1, 4, 1, 8, 1.0, 0, 0, None) == -1   # dw_stride < C
-    assert lib.dpk_rms_norm_backward(p, 8, p, 8, None, 0, p, p, p, p, 8, 1, 4, 0, 8, 1.0, 0, 0, None) == -1   # no part
+    assert lib.dpk_rms_norm_backward(p, 8, None, 0, p, 8, None, 0, p, p, p, p, 7, 1, 4, 1, 8, 1.0, 0, 0, None) == -1   # dw_stride < C
+    assert lib.dpk_rms_norm_backward(p, 8, None, 0, p, 8, None, 0, p, p, p, p, 8, 1, 4, 0, 8, 1.0, 0, 0, None) == -1   # no part
+    assert lib.dpk_rms_norm_backward(p, 8, p, 8, p, 8, None, 0, p, p, p, p, 8, 1, 4, 1, 8, 1.0, 0, 0, None) == -1   # fp32: R is the sum
     conv = lambda x=p, w=p, T=3, D=8, W=4, dt=0: lib.dpk_causal_conv_forward(x, 24, 8, w, None, None, None, p, None, 2, T, D, W, 1, dt, None)  # noqa: E731
     assert conv(x=None) == conv(w=None) == conv(T=-1) == conv(D=0) == conv(W=0) == conv(dt=9) == -1 and conv(W=5) == -2
     assert lib.dpk_causal_conv_step(p, 8, None, p, None, p, 2, 8, 4, 1, 0, None) == -1
