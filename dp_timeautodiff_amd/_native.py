@@ -12,6 +12,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libdpk_gfx950.so"
@@ -901,6 +902,7 @@ def causal_conv_step(x, state, weight, bias, silu: bool):
     if x.stride(1) != 1 and D > 1:
         x = x.contiguous()
     y = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    increment_version(state)  # written behind torch's back: a graph that has saved it must notice
     if B:
         _call("dpk_causal_conv_step", x.device, x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _addr(bias),
               y.data_ptr(), B, D, W, int(silu), ACT_DTYPES[x.dtype])
@@ -1057,6 +1059,7 @@ def selective_scan_step(inp: ScanInputs, state):
     if state is None or _par(state, "state", (b, d, inp.A_log.shape[1]), u.device) is not state:
         raise DpkError("selective_scan_step: the state is updated in place and must be a contiguous [B, D, N]")
     out = torch.empty(b, d, dtype=u.dtype, device=u.device)
+    increment_version(state)
     if b:
         s, _ = inp.desc()
         _call("dpk_selective_scan_step", u.device, ctypes.byref(s), state.data_ptr(), out.data_ptr())

@@ -96,6 +96,8 @@ class DPRMSNorm(nn.Module):
         claim = _active_claim(self)
         if claim is None:
             return rms_norm(x, self.weight, residual, eps=self.eps, quantize=quantize)
+        if x.dim() < 2:
+            raise ValueError(f"per-sample gradients need samples along a dimension of their own, got x of shape {tuple(x.shape)}")
         swap = not claim.batch_first and not self.batch_major and x.dim() >= 3  # samples along dimension 1: the kernel wants a sample's rows together
         if swap:
             x, residual = (None if t is None else t.transpose(0, 1).contiguous() for t in (x, residual))

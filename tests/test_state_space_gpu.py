@@ -517,6 +517,22 @@ def test_forward_and_backward_replay_from_a_graph(shape):
         assert all(torch.equal(a, b) for a, b in zip(static, eager)), k
 
 
+def test_a_step_over_a_state_that_backward_needs_is_noticed():
+    from dp_timeautodiff_amd.layers import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+    x, cs, w, a, h = (t.cuda() for t in make(5, torch.float32, (2, 3, 8), (2, 3, 8), (8, 4), (8, 4), (2, 8, 4)))
+    b = x[..., :4]
+    xg = x.clone().requires_grad_()
+    causal_conv_step(x[:, 0], cs, w)
+    y = causal_conv(xg, w, state=cs)
+    causal_conv_step(x[:, 0], cs, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = selective_scan(xg, x, a, b, b, state=h)
+    selective_scan_step(x[:, 0], x[:, 0], a, b[:, 0], b[:, 0], h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_two_streams_at_once():
     jobs = [_train_inputs(2, 700, 130, seed=k) for k in range(2)]
     want = [_train(*j) for j in jobs]

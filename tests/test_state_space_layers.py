@@ -259,6 +259,14 @@ def test_sequence_first_norm_and_data_as_its_input(dev):
             assert rel_err(v.grad_sample[b].cpu().numpy(), p[n].grad.numpy()) < TOL, n
 
 
+def test_a_single_row_has_no_samples(dev):
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    from dp_timeautodiff_amd.layers import DPRMSNorm
+    gsm = GradSampleModule(DPRMSNorm(8).to(dev))
+    with pytest.raises(ValueError, match="samples"):
+        gsm(torch.randn(8, device=dev))
+
+
 def test_validator_replaces_torch_rms_norm(dev):
     from dp_timeautodiff_amd.grad_sample import GradSampleModule
     from dp_timeautodiff_amd.layers import DPRMSNorm
