@@ -732,10 +732,10 @@ def _dense(t):
 
 
 def _as_btf(t: torch.Tensor):
-    """[B, T, F] whose last dimension is contiguous (and whose rows are less than 2^26 elements apart: the scan's lanes count a
+    """[B, T, F] whose last dimension is contiguous (and whose rows are less than 2^24 elements apart: the scan's lanes count a
     group's rows in 32-bit byte offsets)."""
     s = t.stride()
-    return t if (s[2] == 1 or t.shape[2] == 1) and s[1] < 1 << 26 else t.contiguous()
+    return t if (s[2] == 1 or t.shape[2] == 1) and s[1] < 1 << 24 else t.contiguous()
 
 
 def _sum_rows(device, src: int, groups: int, rows: int, in_stride: int, outs, scale: float, accumulate: bool):

@@ -18,7 +18,7 @@
 // lane swaps.
 // Per state and step: forward one v_exp_f32 (quarter rate) and four plain instructions, backward one and twelve, and the sums
 // over channels for dB and dC, a halving tree over the lanes (four more).  Measured at 256 x 256 x 1024, N = 16, fp32: forward
-// 350 us = 4.5 TB/s with the kept states, backward 955 us, bound by the vector ALU (about 80 % busy), of which 2.4 GB of traffic are
+// 350 us = 4.5 TB/s with the kept states, backward 930 us, bound by the vector ALU (about 80 % busy), of which 2.4 GB of traffic are
 // 500 us.
 // Sequences x channels / 64 is the number of waves; few long sequences are cut into chunks of time: each chunk's effect is
 // (decay, state from zero), which a short kernel joins in order, and the chunks then run side by side from their true states.
@@ -83,17 +83,47 @@ struct Staged {
     static constexpr int K = GROUP * 2 * NT > 256 ? GROUP * 2 * NT / 256 : 1;
     float v[K];
 };
+// Operands are read and written relative to their group's first row: a 64-bit address that the wave shares and a 32-bit byte offset
+// a lane.  GLOBAL: a store that the compiler takes for a flat one would be waited for with the next access to LDS.
+#define GLOBAL __attribute__((address_space(1)))
+template <typename T>
+__device__ __forceinline__ const char* group_row(const void* p, int64_t sb, int64_t st, int b, int t0) {
+    return (const char*)p + (b * sb + t0 * st) * (int64_t)sizeof(T);
+}
+// rows of one sequence
+template <typename T>
+struct Rows {
+    const char* first;
+    uint32_t st;
+    __device__ __forceinline__ Rows(const void* p, int64_t sb, int64_t st_, int b) : first((const char*)p + b * sb * (int64_t)sizeof(T)), st((uint32_t)st_) {
+        asm("" : "+s"(first));
+    }
+    __device__ __forceinline__ const char* at(int t0) const { return first + (uint64_t)(uint32_t)t0 * st * sizeof(T); }
+};
+__device__ __forceinline__ char* out_row(void* p, int64_t at) {
+    char* r = (char*)p + at;
+    asm("" : "+s"(r));   // (else the lane's offset is added first and the row's becomes a 64-bit product per lane)
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float at(const char* row, uint32_t bytes) {
+    return to_f32(*(GLOBAL const T*)(row + bytes));
+}
+template <typename T>
+__device__ __forceinline__ void put(char* row, uint32_t bytes, float v) {
+    *(GLOBAL T*)(row + bytes) = (T)v;
+}
+
 template <typename T, int NT>
-__device__ __forceinline__ void fetch_bc(const ScanArgs& a, int b, int t0, int end, Staged<NT>& r) {
+__device__ __forceinline__ void fetch_bc(const ScanArgs& a, const Rows<T>& rb, const Rows<T>& rc, int t0, int end, Staged<NT>& r) {
     if (blockDim.x != 256) return;
+    const char *gb = rb.at(t0), *gc = rc.at(t0);
 #pragma unroll
     for (int k = 0; k < Staged<NT>::K; ++k) {
         const int i = threadIdx.x + k * 256;
         const int q = i / (2 * NT), c = i % (2 * NT), n = c % NT;
-        r.v[k] = 0.f;
-        if (i < GROUP * 2 * NT && t0 + q < end && n < a.N)
-            r.v[k] = c < NT ? to_f32(((const T*)a.B)[(int64_t)b * a.B_sb + (int64_t)(t0 + q) * a.B_st + n])
-                            : to_f32(((const T*)a.C)[(int64_t)b * a.C_sb + (int64_t)(t0 + q) * a.C_st + n]);
+        const uint32_t row = i < GROUP * 2 * NT && t0 + q < end ? q : 0, col = n < a.N ? n : 0;   // others read and put 0
+        r.v[k] = at<T>(c < NT ? gb : gc, (__umul24(row, c < NT ? rb.st : rc.st) + col) * (uint32_t)sizeof(T));
     }
 }
 template <typename T, int NT>
@@ -105,22 +135,8 @@ __device__ __forceinline__ void put_bc(const ScanArgs& a, int b, int t0, int end
 #pragma unroll
     for (int k = 0; k < Staged<NT>::K; ++k) {
         const int i = threadIdx.x + k * 256;
-        if (i < GROUP * 2 * NT) (&s[0][0])[i] = r.v[k];
+        if (i < GROUP * 2 * NT) (&s[0][0])[i] = t0 + i / (2 * NT) < end && i % NT < a.N ? r.v[k] : 0.f;
     }
-}
-
-// Operands are read relative to their group's first row: a 64-bit address that the wave shares and a 32-bit byte offset a lane.
-template <typename T>
-__device__ __forceinline__ const char* group_row(const void* p, int64_t sb, int64_t st, int b, int t0) {
-    return (const char*)p + (b * sb + t0 * st) * (int64_t)sizeof(T);
-}
-template <typename T>
-__device__ __forceinline__ float at(const char* row, uint32_t bytes) {
-    return to_f32(*reinterpret_cast<const T*>(row + bytes));
-}
-template <typename T>
-__device__ __forceinline__ void put(char* row, uint32_t bytes, float v) {
-    *reinterpret_cast<T*>(row + bytes) = (T)v;
 }
 
 template <typename T>
@@ -385,28 +401,11 @@ __device__ __forceinline__ void fold_dpp(float* v) {
     }
 }
 constexpr int half_of(int c) { return c > 1 ? c / 2 : 1; }
-// Four values over the 64 / LS low lanes.  At N = 16 (LS = 4) the halving is by DPP adds that write only the banks (four lanes) a value
-// stays on, which the compiler does not form from a choice and an add (11 instructions: 985 us at 256 x 256 x 1024, 950 so).  A
-// DPP operand may be read two wait states after its write: the s_nops, with the independent adds between them, keep that.
+// Four values each of two steps over the 64 / LS low lanes.  At N = 16 (LS = 4) the halving is by DPP adds that write only the banks
+// (four lanes) a value stays on, which the compiler does not form from a choice and an add.  A DPP operand may be read two wait
+// states after its write: the other step's adds and the s_nops keep that.
 template <int LS>
 __device__ __forceinline__ float lane_sums(float (&v)[4]) {
-    if constexpr (LS == 4) {
-        float a, b, r;
-        asm("s_nop 1\n\t"
-            "v_add_f32_dpp %0, %3, %3 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
-            "v_add_f32_dpp %1, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
-            "v_add_f32_dpp %0, %5, %5 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-            "v_add_f32_dpp %1, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-            "s_nop 0\n\t"
-            "v_add_f32_dpp %2, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
-            "v_add_f32_dpp %2, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-            "s_nop 1\n\t"
-            "v_add_f32_dpp %0, %2, %2 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
-            "s_nop 1\n\t"
-            "v_add_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf"
-            : "=&v"(a), "=&v"(b), "=&v"(r) : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]));
-        return a;
-    }
     constexpr int C1 = LS == 1 ? 2 : 4, C2 = LS <= 2 ? half_of(C1) : 4, C3 = LS <= 4 ? half_of(C2) : 4;
     constexpr int C4 = half_of(C3), C5 = half_of(C4);
     if constexpr (LS == 1) fold32<4>(v);
@@ -416,6 +415,38 @@ __device__ __forceinline__ float lane_sums(float (&v)[4]) {
     fold_dpp<C4, 0x4E, 2>(v);                           // quad_perm 2,3,0,1
     fold_dpp<C5, 0xB1, 1>(v);                           // quad_perm 1,0,3,2
     return v[0];
+}
+template <int LS>
+__device__ __forceinline__ void lane_sums(float (&v)[2][4], float& s0, float& s1) {
+    if constexpr (LS == 4) {
+        float a, b, c, d, r, s;
+        asm("s_nop 1\n\t"
+            "v_add_f32_dpp %0, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %1, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %2, %10, %10 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %3, %11, %11 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %0, %8, %8 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+            "v_add_f32_dpp %1, %9, %9 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+            "v_add_f32_dpp %2, %12, %12 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+            "v_add_f32_dpp %3, %13, %13 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+            "v_add_f32_dpp %4, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %4, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+            "v_add_f32_dpp %5, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %5, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+            "s_nop 0\n\t"
+            "v_add_f32_dpp %0, %4, %4 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %2, %5, %5 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+            "s_nop 0\n\t"
+            "v_add_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+            "v_add_f32_dpp %2, %2, %2 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf"
+            : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(r), "=&v"(s)
+            : "v"(v[0][0]), "v"(v[0][1]), "v"(v[0][2]), "v"(v[0][3]), "v"(v[1][0]), "v"(v[1][1]), "v"(v[1][2]), "v"(v[1][3]));
+        s0 = a;
+        s1 = c;
+    } else {
+        s0 = lane_sums<LS>(v[0]);
+        s1 = lane_sums<LS>(v[1]);
+    }
 }
 template <int LS>
 __device__ __forceinline__ int lane_slot(int lane) {   // which of the four values the lane ends up with
@@ -522,26 +553,34 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
     float nu[OWN], npre[OWN], ndy[OWN], nz[OWN], nh[S];
     Staged<NT> nbc;
     const uint32_t lane_out = ((uint32_t)q0 * a.D + d) * sizeof(T);
+    const uint32_t out_step = (uint32_t)a.D * sizeof(T);
+    char *du_b = out_row(a.du, (int64_t)b * a.T * out_step), *dd_b = out_row(a.ddelta, (int64_t)b * a.T * out_step);
+    // sums over this workgroup's channels: dB and dC themselves, or one row of both for every channel block
+    const bool blocks = a.ndb > 1;
+    const uint32_t sum_step = blocks ? 8u * a.N : (uint32_t)a.N * sizeof(T);
+    char* sums_b = blocks ? out_row(a.dbc, ((int64_t)dblk * a.nb + b) * a.T * sum_step) : out_row(a.dB, (int64_t)b * a.T * sum_step);
+    char* dc_b = out_row(a.dC, (int64_t)b * a.T * sum_step);   // (not used with channel blocks)
+    char* dz_b = out_row(a.dz, (int64_t)b * a.T * out_step);
     const bool gate = a.dz != nullptr;   // without a gate a.z is a.u: read, and not used
     const uint32_t lane_kept = ((uint32_t)n0 * a.D + dd) * 4u;
+    const Rows<T> ru(a.u, a.u_sb, a.u_st, b), rd(a.delta, a.delta_sb, a.delta_st, b), ro(a.dout, a.dout_sb, a.dout_st, b);
+    const Rows<T> rz(a.z, a.z_sb, a.z_st, b), rb(a.B, a.B_sb, a.B_st, b), rc(a.C, a.C_sb, a.C_st, b);
+    const float* kept_b = a.kept + (int64_t)b * ngroup * NT * a.D;
     auto fetch = [&](int t0) {
-        const char* gu = group_row<T>(a.u, a.u_sb, a.u_st, b, t0);
-        const char* gd = group_row<T>(a.delta, a.delta_sb, a.delta_st, b, t0);
-        const char* go = group_row<T>(a.dout, a.dout_sb, a.dout_st, b, t0);
-        const char* gz = group_row<T>(a.z, a.z_sb, a.z_st, b, t0);
-        uint32_t q = q0;
-        asm volatile("" : "+v"(q));   // offsets are made here: held over the group they would be spilled, and waited for
+        const char *gu = ru.at(t0), *gd = rd.at(t0), *go = ro.at(t0), *gz = rz.at(t0);
+        uint32_t q = q0, kept = lane_kept;
+        asm volatile("" : "+v"(q), "+v"(kept));   // offsets are made here: held over the group they would be spilled, and waited for
 #pragma unroll
         for (int i = 0; i < OWN; ++i) {
             const uint32_t r = (int)(t0 + q + i) < end ? q + i : 0u;
-            nu[i] = at<T>(gu, (r * (uint32_t)a.u_st + dd) * (uint32_t)sizeof(T));
-            npre[i] = at<T>(gd, (r * (uint32_t)a.delta_st + dd) * (uint32_t)sizeof(T));
-            ndy[i] = at<T>(go, (r * (uint32_t)a.dout_st + dd) * (uint32_t)sizeof(T));
-            nz[i] = at<T>(gz, (r * (uint32_t)a.z_st + dd) * (uint32_t)sizeof(T));
+            nu[i] = at<T>(gu, (__umul24(r, ru.st) + dd) * (uint32_t)sizeof(T));
+            npre[i] = at<T>(gd, (__umul24(r, rd.st) + dd) * (uint32_t)sizeof(T));
+            ndy[i] = at<T>(go, (__umul24(r, ro.st) + dd) * (uint32_t)sizeof(T));
+            nz[i] = at<T>(gz, (__umul24(r, rz.st) + dd) * (uint32_t)sizeof(T));
         }
-        const char* k = (const char*)(a.kept + ((int64_t)b * ngroup + (t0 > k0 ? (t0 - k0) / GROUP : 0)) * NT * a.D);
+        const char* k = (const char*)(kept_b + (int64_t)(t0 > k0 ? (t0 - k0) / GROUP : 0) * (NT * a.D));
 #pragma unroll
-        for (int j = 0; j < S; ++j) nh[j] = at<float>(k, lane_kept + (uint32_t)j * (uint32_t)a.D * 4u);
+        for (int j = 0; j < S; ++j) nh[j] = at<float>(k, kept + (uint32_t)j * (uint32_t)a.D * 4u);
     };
     int t0 = lo + (hi - lo - 1) / GROUP * GROUP;
     for (; t0 >= lo && t0 >= end; t0 -= GROUP) {   // groups behind the sequence
@@ -568,7 +607,7 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
     }
     if (t0 >= lo) {
         fetch(t0);
-        fetch_bc<T, NT>(a, b, t0, end, nbc);
+        fetch_bc<T, NT>(a, rb, rc, t0, end, nbc);
         put_bc<T, NT>(a, b, t0, end, nbc, bc[ph]);
         __syncthreads();
     }
@@ -579,7 +618,8 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
         const int next = t0 - GROUP >= lo ? t0 - GROUP : t0;   // (the first group is fetched twice)
         uint32_t to = lane_out;
         asm volatile("" : "+v"(to));
-        fetch_bc<T, NT>(a, b, next, end, nbc);
+        const int64_t out_at = (int64_t)t0 * a.D * (int64_t)sizeof(T);
+        fetch_bc<T, NT>(a, rb, rc, next, end, nbc);
         {
         {
             float xs[OWN];
@@ -603,13 +643,14 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
         }
         // Steps are kept apart for the scheduler, which would otherwise fetch all of a group's B and C at once.
         {
-            float h[S];
+            float h[S], v[2][S];
+            int first_state = live ? n0 : a.N;
+            asm volatile("" : "+v"(first_state));   // compared here: masks held over the loop are scalar registers spilled
 #pragma unroll
-            for (int j = 0; j < S; ++j) h[j] = n0 + j < a.N && live && t0 >= k0 ? nh[j] : 0.f;
+            for (int j = 0; j < S; ++j) h[j] = first_state + j < a.N && t0 >= k0 ? nh[j] : 0.f;
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
                 __builtin_amdgcn_sched_barrier(0);
-                float v[S];
                 y[q] = 0.f;
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
@@ -617,9 +658,9 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
                     eh[q][j] = e[q][j] * h[j];
                     h[j] = eh[q][j] + x[q] * bc[ph][q][n0 + j];
                     y[q] += bc[ph][q][NT + n0 + j] * h[j];
-                    v[j] = g[q] * h[j];
+                    v[q & 1][j] = g[q] * h[j];
                 }
-                part[ph][wave][q][NT + part_slot] = lane_sums<LS>(v);
+                if (q & 1) lane_sums<LS>(v, part[ph][wave][q - 1][NT + part_slot], part[ph][wave][q][NT + part_slot]);
                 if (q >= GROUP / 2) pair<LS>(y, q - GROUP / 2);   // lanes that hold the same sum write it to the same place
             }
         }
@@ -628,22 +669,21 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
                 const int t = t0 + q0 + i;
-                if (live && t < hi)
-                    put<T>((char*)a.dz + ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T), to, t < end ? zf[i] * (y[i] + skip * u[i]) : 0.f);
+                if (live && t < hi) put<T>(out_row(dz_b, out_at), to + i * out_step, t < end ? zf[i] * (y[i] + skip * u[i]) : 0.f);
             }
         }
+        float v[2][S];
         asm volatile("" ::: "memory");   // B and C are read from LDS again rather than held for all steps
 #pragma unroll
         for (int q = GROUP - 1; q >= 0; --q) {
             __builtin_amdgcn_sched_barrier(0);
             // half of the group's registers are free again: the next group's operands come in behind the other half
             if (q == GROUP / 2 - 1) fetch(next);
-            float v[S];
             into[q] = along[q] = 0.f;
 #pragma unroll
             for (int j = 0; j < S; ++j) {
                 dh[j] += g[q] * bc[ph][q][NT + n0 + j];
-                v[j] = dh[j] * x[q];
+                v[q & 1][j] = dh[j] * x[q];
                 into[q] += dh[j] * bc[ph][q][n0 + j];
                 const float t = dh[j] * eh[q][j];
                 along[q] += t * A2[j];
@@ -651,7 +691,7 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
                 dh[j] *= e[q][j];
                 asm volatile("" : "+v"(dA[j]));   // summed here, not behind the group with eight steps' t held until then
             }
-            part[ph][wave][q][part_slot] = lane_sums<LS>(v);
+            if (!(q & 1)) lane_sums<LS>(v, part[ph][wave][q][part_slot], part[ph][wave][q + 1][part_slot]);
             if (q < GROUP / 2) {
                 pair<LS>(into, q);
                 pair<LS>(along, q);
@@ -672,26 +712,25 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
             const float dpre = (into[i] * u[i] + along[i] * LN2) * slope[i];
             if (in) dbias += dpre;
             if (live && t < hi) {
-                const int64_t o = ((int64_t)b * a.T + t0 + i) * a.D * (int64_t)sizeof(T);
-                put<T>((char*)a.du + o, to, in ? into[i] * dts[i] + skip * gs[i] : 0.f);
-                put<T>((char*)a.ddelta + o, to, in ? dpre : 0.f);
+                put<T>(out_row(du_b, out_at), to + i * out_step, in ? into[i] * dts[i] + skip * gs[i] : 0.f);
+                put<T>(out_row(dd_b, out_at), to + i * out_step, in ? dpre : 0.f);
             }
         }
         }
         __syncthreads();   // the group's sums are written, the next group's B and C staged
+        char* sums = out_row(sums_b, (int64_t)t0 * sum_step);
+        char* sums_c = blocks ? sums : out_row(dc_b, (int64_t)t0 * sum_step);
         for (int i = threadIdx.x; i < GROUP * 2 * NT; i += blockDim.x) {
             const int q = i / (2 * NT), r = i % (2 * NT), n = r % NT;
             if (n >= a.N || t0 + q >= hi) continue;
             float s = 0.f;
             if (t0 + q < end)
                 for (int w = 0; w < nw; ++w) s += part[ph][w][q][r];
-            const int64_t bt = (int64_t)b * a.T + t0 + q;
-            if (a.ndb > 1)
-                a.dbc[((int64_t)dblk * a.nb * a.T + bt) * 2 * a.N + (r < NT ? n : a.N + n)] = s;
-            else if (r < NT)
-                ((T*)a.dB)[bt * a.N + n] = (T)s;
+            const uint32_t row = __umul24(q, sum_step);
+            if (blocks)
+                put<float>(sums, row + (r < NT ? n : a.N + n) * 4u, s);
             else
-                ((T*)a.dC)[bt * a.N + n] = (T)s;
+                put<T>(r < NT ? sums : sums_c, row + n * (uint32_t)sizeof(T), s);
         }
         ph ^= 1;
     }
@@ -789,10 +828,10 @@ int check(const dpk_scan_desc* s) {
     if (s->u_sb < 0 || s->u_st < 0 || s->delta_sb < 0 || s->delta_st < 0 || s->B_sb < 0 || s->B_st < 0 || s->C_sb < 0 ||
         s->C_st < 0 || s->z_sb < 0 || s->z_st < 0)
         return DPK_EINVAL;
-    // a lane's byte offset within a group of rows is 32 bits
-    const int64_t row_limit = (int64_t)1 << 26;
+    // a lane's byte offset within a group of rows is 32 bits, a product with a row's distance takes 24 of it (at the full rate)
+    const int64_t row_limit = (int64_t)1 << 24;
     if (s->D >= row_limit || (int64_t)s->D * s->N >= (int64_t)1 << 29 || s->u_st >= row_limit || s->delta_st >= row_limit ||
-        s->z_st >= row_limit)
+        s->z_st >= row_limit || s->B_st >= row_limit || s->C_st >= row_limit)
         return DPK_ERANGE;
     if (!s->A_log || (s->T > 0 && (!s->u || !s->delta || !s->Bm || !s->Cm))) return DPK_EINVAL;
     const int bl = block_of(s->D);
@@ -878,7 +917,7 @@ extern "C" int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_sca
     const int rc = check(s);
     if (rc) return rc;
     if (!g || g->dout_sb < 0 || g->dout_st < 0) return DPK_EINVAL;
-    if (g->dout_st >= (int64_t)1 << 26) return DPK_ERANGE;
+    if (g->dout_st >= (int64_t)1 << 24) return DPK_ERANGE;
     if (s->B == 0) return DPK_OK;
     if (s->T > 0 && (!g->dout || !g->du || !g->ddelta || !g->dB || !g->dC || !s->kept || (s->z && !g->dz))) return DPK_EINVAL;
     if (s->nchunk > 1 && (!s->edge || !s->span)) return DPK_EINVAL;

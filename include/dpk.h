@@ -372,7 +372,7 @@ int dpk_causal_conv_step(const void* x, int64_t x_sb, void* state, const float* 
 /*
  * K14: dt = softplus(delta + dt_bias) (softplus = 0: the sum itself), A = -exp(A_log) [D,N], h_t = exp(dt A) h_{t-1} + dt Bm_t u_t,
  * y = Cm_t . h_t + Dskip u_t, out = y silu(z).  u, delta, z [B,T,D], Bm, Cm [B,T,N], N <= DPK_SCAN_MAX_STATE; Dskip, z, dt_bias, h0
- * [B,D,N], lengths [B] may be NULL.  Rows at and behind lengths[b] leave the state alone and give out = 0.
+ * [B,D,N], lengths [B] may be NULL.  Rows are less than 2^24 elements apart.  Rows at and behind lengths[b] leave the state alone and give out = 0.
  * kept: [B, G, dpk_selective_scan_state_rows(N), D] floats, written by forward where the backward pass is to follow (else NULL); G =
  * ceil(T / dpk_selective_scan_group()), without h0 one less, but at least 1.
  * nchunk, chunk: as dpk_selective_scan_chunks says (or 1 and T rounded up to the group); nchunk > 1 needs edge

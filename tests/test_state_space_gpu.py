@@ -418,7 +418,22 @@ def test_offsets_past_32_bits():
     rows.copy_(dense[0])
     assert torch.equal(selective_scan(rows, dense[1], dense[2], dense[3], dense[4]), selective_scan(*dense[:5]))
     assert torch.equal(causal_conv(rows, w), causal_conv(dense[0], w))
-    del u, delta, z, rows, buf
+    # rows just inside and just outside what the lanes' offsets reach, of every operand and of the gradient
+    small, _, _, _ = scan_inputs((1, T, D, N, "zdbs", None), torch.bfloat16)
+    small = [None if t is None else t.cuda() for t in small[:8]]
+    want = [t.clone().requires_grad_() for t in (small[0], small[1], small[3], small[4], small[6])]
+    dy = make(9, torch.bfloat16, (1, T, D))[0].cuda()
+    selective_scan(want[0], want[1], small[2], want[2], want[3], small[5], want[4], small[7]).backward(dy)
+    for step in (2 ** 24 - 1, 2 ** 24):
+        def wide(t, at):
+            v = buf.as_strided((1, T, t.shape[2]), (1, step, 1), at)
+            v.copy_(t)
+            return v
+        dout = wide(dy, 64 * 5)
+        got = [wide(t.detach(), 64 * i).requires_grad_() for i, t in enumerate(want)]
+        selective_scan(got[0], got[1], small[2], got[2], got[3], small[5], got[4], small[7]).backward(dout)
+        assert all(torch.equal(g.grad, w.grad) for g, w in zip(got, want)), step
+    del u, delta, z, rows, buf, got
     x = torch.empty(2 ** 24 + 3, 130, dtype=torch.bfloat16, device="cuda").fill_(1.5)  # 2.2e9 elements
     x[-1] = make(2, torch.bfloat16, (130,))[0].cuda()
     y, _ = rms_norm(x, torch.ones(130, device="cuda"))

@@ -394,6 +394,7 @@ def test_c_entry_refusals():
         return lib.dpk_selective_scan_forward(ctypes.byref(scan(**k)), out, None, None)
 
     assert fwd(out=None) == fwd(u=None) == fwd(A_log=None) == fwd(D=0) == fwd(N=0) == fwd(T=-1) == fwd(dtype=5) == fwd(u_sb=-1) == -1
+    assert fwd(u_st=1 << 24) == fwd(z_st=1 << 24) == fwd(B_st=1 << 24) == fwd(C_st=1 << 24) == -2   # a lane's offsets would not reach
     assert fwd(N=33) == -2 and fwd(nchunk=0) == fwd(chunk=12) == fwd(chunk=8) == fwd(nchunk=2) == -1   # chunks that miss rows, no scratch
     g = _native._ScanGrads()
     assert lib.dpk_selective_scan_backward(ctypes.byref(scan()), ctypes.byref(g), None) == -1
