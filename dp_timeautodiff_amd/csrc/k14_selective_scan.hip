@@ -260,16 +260,18 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_forward_kernel(Sca
     }
 }
 
+constexpr int JOIN_RUN = 8;
 // Joins the chunks: edge[c] comes in as what chunk c makes of a zero start and goes out as its true start (forward) or the
-// gradient that enters it from behind (reverse).  Eight lanes share a state: each takes a run of eight chunks into registers, the
-// runs' (decay, state from zero) are joined by lane shuffles, and each lane walks its run again from its true start.
-template <bool REVERSE>
+// gradient that enters it from behind (reverse).  LANES lanes share a state: each takes a run of eight chunks into registers, the
+// runs' (decay, state from zero) are joined by lane shuffles, and each lane walks its run again from its true start.  As many lanes
+// as there are runs, up to eight: the wave's other lanes are neighbouring states, so fewer runs make longer runs of memory (5 chunks
+// of 50 x 16 x 1024 states: 79 us with eight lanes, 13 with one).
+template <bool REVERSE, int LANES>
 __global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs a) {
-    constexpr int RUN = 8, LANES = 8;
+    constexpr int RUN = JOIN_RUN, STATES = 64 / LANES;
     const int64_t per = (int64_t)a.N * a.D;
-    // 8 neighbouring states and 8 runs a wave: lane = run * 8 + state
-    const int run = (threadIdx.x & 63) >> 3;
-    const int64_t i = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 8 + (threadIdx.x & 7);
+    const int run = (threadIdx.x & 63) / STATES, state = threadIdx.x % STATES;
+    const int64_t i = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * STATES + state;
     const bool live = i < a.nb * per;
     const int64_t at = live ? i : 0;
     const int b = (int)(at / per);
@@ -297,15 +299,19 @@ __global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs a) {
         }
 #pragma unroll
         for (int off = 1; off < LANES; off <<= 1) {   // joined with all runs before it
-            const float pf = __shfl_up(f, 8 * off, 64), pz = __shfl_up(z, 8 * off, 64);
+            const float pf = __shfl_up(f, STATES * off, 64), pz = __shfl_up(z, STATES * off, 64);
             if (run >= off) {
                 z = z + f * pz;
                 f *= pf;
             }
         }
-        const float pf = __shfl_up(f, 8, 64), pz = __shfl_up(z, 8, 64);
+        float pf = 1.f, pz = 0.f;
+        if constexpr (LANES > 1) {
+            pf = __shfl_up(f, STATES, 64);
+            pz = __shfl_up(z, STATES, 64);
+        }
         float g = run ? pz + pf * h : h;
-        const float lf = __shfl(f, 56 + (threadIdx.x & 7), 64), lz = __shfl(z, 56 + (threadIdx.x & 7), 64);
+        const float lf = __shfl(f, 64 - STATES + state, 64), lz = __shfl(z, 64 - STATES + state, 64);
         h = lz + lf * h;
 #pragma unroll
         for (int k = 0; k < RUN; ++k) {
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs a) {
 
 // what a chunk hands to the chunk before it if nothing enters it from behind
 template <typename T, int NT>
-__global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_backward_edge_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(256, 2) scan_backward_edge_kernel(ScanArgs a) {
     __shared__ float bc[2][GROUP][2 * NT];
     const Place p(a);
     const int end = seq_end(a, p.b);
@@ -333,10 +339,7 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_backward_edge_kern
     const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f;
     const uint32_t lane_in = (uint32_t)dd * sizeof(T);
     float span = 0.f;
-    int ph = 0;
-    for (int t0 = p.t0 + (p.t1 - p.t0 - 1) / GROUP * GROUP; t0 >= p.t0; t0 -= GROUP) {
-        if (t0 >= end) continue;
-        float dy[GROUP], dt[GROUP], z[GROUP];
+    auto fetch = [&](int t0, float (&dt)[GROUP], float (&dy)[GROUP], float (&z)[GROUP]) {
         const char* gd = group_row<T>(a.delta, a.delta_sb, a.delta_st, p.b, t0);
         const char* go = group_row<T>(a.dout, a.dout_sb, a.dout_st, p.b, t0);
         const char* gz = group_row<T>(a.z, a.z_sb, a.z_st, p.b, t0);
@@ -347,7 +350,28 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_backward_edge_kern
             dy[q] = at<T>(go, lane_in + r * (uint32_t)a.dout_st);
             z[q] = at<T>(gz, lane_in + r * (uint32_t)a.z_st);
         }
-        stage_bc<T, NT>(a, p.b, t0, end, bc[ph]);
+    };
+    const Rows<T> rb(a.B, a.B_sb, a.B_st, p.b), rc(a.C, a.C_sb, a.C_st, p.b);
+    float ndt[GROUP], ndy[GROUP], nz[GROUP];
+    Staged<NT> nbc;
+    int ph = 0, t0 = p.t0 + (p.t1 - p.t0 - 1) / GROUP * GROUP;
+    while (t0 >= p.t0 && t0 >= end) t0 -= GROUP;
+    if (t0 >= p.t0) {
+        fetch(t0, ndt, ndy, nz);
+        fetch_bc<T, NT>(a, rb, rc, t0, end, nbc);
+    }
+    for (; t0 >= p.t0; t0 -= GROUP) {
+        float dy[GROUP], dt[GROUP], z[GROUP];
+#pragma unroll
+        for (int q = 0; q < GROUP; ++q) {
+            dt[q] = ndt[q];
+            dy[q] = ndy[q];
+            z[q] = nz[q];
+        }
+        put_bc<T, NT>(a, p.b, t0, end, nbc, bc[ph]);
+        const int next = t0 - GROUP >= p.t0 ? t0 - GROUP : t0;   // (the first group is fetched twice)
+        fetch(next, ndt, ndy, nz);
+        fetch_bc<T, NT>(a, rb, rc, next, end, nbc);
         __syncthreads();
 #pragma unroll
         for (int q = GROUP - 1; q >= 0; --q) {
@@ -855,6 +879,19 @@ ScanArgs fill(const dpk_scan_desc* s) {
     return a;
 }
 
+template <bool REVERSE>
+void join(const ScanArgs& a, hipStream_t st) {
+    const int64_t states = (int64_t)a.nb * a.N * a.D;
+#define CALL(LANES)                                                                                                             \
+    hipLaunchKernelGGL((scan_join_kernel<REVERSE, LANES>), dim3((unsigned)((states + 256 / LANES - 1) / (256 / LANES))), dim3(256), \
+                       0, st, a)
+    if (a.nchunk <= JOIN_RUN) CALL(1);
+    else if (a.nchunk <= 2 * JOIN_RUN) CALL(2);
+    else if (a.nchunk <= 4 * JOIN_RUN) CALL(4);
+    else CALL(8);
+#undef CALL
+}
+
 }  // namespace
 
 #define SCAN_N(N, CALL)           \
@@ -864,16 +901,18 @@ ScanArgs fill(const dpk_scan_desc* s) {
     else { CALL(32) }
 
 // Chunks of time a scan is cut into.  Cutting costs a second reading of the inputs and most of the arithmetic again, so it has to
-// win a factor of two in waves at least: only scans of fewer than 512 waves (half a wave a SIMD) are cut, into up to 2048 waves.
-// Forward, chunks may be as short as 32 steps (2 x 4096 x 500, N = 16, bf16: 75 us against 102 with 64), backward 64 (145 us
-// against 154 with 32: its waves hold 16 channels, so there are four times as many to begin with).
+// win a factor of two or three in waves.  Forward into up to 4096 waves (four a SIMD; 1 x 8192 x 1024, N = 16, bf16: 93 us against
+// 100 with 2048) of chunks as short as 32 steps (2 x 4096 x 500: 75 us against 102 with 64), from fewer than 1366 (8 x 1000 x 4096
+// bf16: 323 us against 917 in one piece; 20 x 1000 x 4096: 744 against 918), of short sequences fewer than 512 (50 x 256 x 1024
+// fp32: 134 against 127).  Backward into up to 2048 of at least 64 steps (145 us against 154 with 32: its waves hold 16 channels,
+// so there are four times as many to begin with) from fewer than 512 (8 x 1000 x 4096: 690 us against 643).
 extern "C" int dpk_selective_scan_chunks(int B, int T, int D, int backward, int* chunk) {
     if (B <= 0 || T <= 0 || D <= 0) {
         if (chunk) *chunk = (T > 0 ? (T + GROUP - 1) / GROUP * GROUP : 0);
         return 1;
     }
     const int64_t waves = (int64_t)B * ((D + 63) / 64);
-    int64_t n = waves >= 512 ? 1 : 2048 / waves;
+    int64_t n = waves >= (backward || T < 512 ? 512 : 1366) ? 1 : (backward ? 2048 : 4096) / waves;
     const int shortest = backward ? 64 : 32;
     const int64_t most = (T + shortest - 1) / shortest;
     if (n > most) n = most;
@@ -905,7 +944,7 @@ extern "C" int dpk_selective_scan_forward(const dpk_scan_desc* s, void* out, flo
 #define CALL(NT) hipLaunchKernelGGL((scan_forward_kernel<E, NT, true>), grid, block, 0, st, a);
         DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
 #undef CALL
-        hipLaunchKernelGGL(scan_join_kernel<false>, dim3((unsigned)(((int64_t)a.nb * a.N * a.D + 31) / 32)), dim3(256), 0, st, a);
+        join<false>(a, st);
     }
 #define CALL(NT) hipLaunchKernelGGL((scan_forward_kernel<E, NT, false>), grid, block, 0, st, a);
     DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
@@ -937,7 +976,7 @@ extern "C" int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_sca
 #define CALL(NT) hipLaunchKernelGGL((scan_backward_edge_kernel<E, NT>), grid, block, 0, st, a);
         DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
 #undef CALL
-        hipLaunchKernelGGL(scan_join_kernel<true>, dim3((unsigned)(((int64_t)a.nb * a.N * a.D + 31) / 32)), dim3(256), 0, st, a);
+        join<true>(a, st);
     }
     a.ndb = blocks;
     const dim3 bgrid((unsigned)(a.nb * a.nchunk * a.ndb)), bblock((unsigned)back_block_of(a.D, a.N));

@@ -198,7 +198,8 @@ SCAN = [  # B, T, D, N, options: z gate, d skip, b bias, s softplus, h state; le
     (2, 21, 40, 32, "zdbsh", [21, 16]), (2, 10, 30, 8, "dbh", None), (2, 0, 5, 4, "zdbsh", None), (0, 3, 5, 4, "zdbs", None),
     (2, 1000, 70, 16, "zdbsh", [1000, 130]), (1, 650, 257, 4, "zds", None), (5, 5, 256, 16, "zdbs", None),
     (1, 700, 40, 16, "sh", [611]), (1, 500, 20, 32, "zdbsh", None), (1, 9001, 3, 7, "zdbsh", None), (3, 300, 8, 8, "bs", [300, 0, 64]),
-    (700, 3, 240, 16, "zdbsh", None), (901, 9, 300, 4, "zdbs", [9, 0, 5] * 300 + [2])]
+    (700, 3, 240, 16, "zdbsh", None), (901, 9, 300, 4, "zdbs", [9, 0, 5] * 300 + [2]),
+    (520, 530, 3, 2, "zbsh", [530, 77, 333, 0] * 130), (1, 1300, 20, 3, "zdsh", None), (70, 200, 250, 5, "zds", None)]   # the first and last: forward in 7 chunks each
 
 
 def scan_inputs(case, dtype, seed=0):
