@@ -38,7 +38,7 @@ struct ScanArgs {
     float *dbc;                 // [d block][b][t][2N] partial sums of dB | dC, where a row of channels needs several workgroups
     float *dA, *dD, *dbias;     // parameter gradients, row (b * nchunk + chunk) of par_stride floats
     int64_t u_sb, u_st, delta_sb, delta_st, B_sb, B_st, C_sb, C_st, z_sb, z_st, dout_sb, dout_st, par_stride;
-    int nb, T, D, N, softplus, nchunk, chunk, ndb, accumulate;
+    int nb, T, D, N, softplus, gate, nchunk, chunk, ndb, accumulate;   // without a gate z is u: read, and not used
     float scale;
 };
 
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_forward_kernel(Sca
                 const uint32_t r = t0 + q < end ? q * (uint32_t)sizeof(T) : 0u;   // rows behind the sequence: the group's first
                 u[q] = at<T>(gu, lane_in + r * (uint32_t)a.u_st);
                 dt[q] = at<T>(gd, lane_in + r * (uint32_t)a.delta_st);
-                if (!EDGE && a.z) z[q] = at<T>(gz, lane_in + r * (uint32_t)a.z_st);
+                if (!EDGE) z[q] = at<T>(gz, lane_in + r * (uint32_t)a.z_st);   // (with a gate or not: in a branch it is waited for)
             }
             stage_bc<T, NT>(a, p.b, t0, end, bc[ph]);
             __syncthreads();
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256, NT <= 16 ? 4 : 2) scan_forward_kernel(Sca
                     if (!EDGE) y += bc[ph][q][NT + n] * h[n];
                 }
                 if (!EDGE) {
-                    if (a.z) y *= z[q] * sigmoid_f(z[q]);
+                    if (a.gate) y *= z[q] * sigmoid_f(z[q]);
                     if (p.live && t0 + q < p.t1) put<T>(out + (int64_t)q * a.D * (int64_t)sizeof(T), lane_out, t0 + q < end ? y : 0.f);
                 }
             }
@@ -585,9 +585,9 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
     char* sums_b = blocks ? out_row(a.dbc, ((int64_t)dblk * a.nb + b) * a.T * sum_step) : out_row(a.dB, (int64_t)b * a.T * sum_step);
     char* dc_b = out_row(a.dC, (int64_t)b * a.T * sum_step);   // (not used with channel blocks)
     char* dz_b = out_row(a.dz, (int64_t)b * a.T * out_step);
-    const bool gate = a.dz != nullptr;   // without a gate a.z is a.u: read, and not used
     const uint32_t lane_kept = ((uint32_t)n0 * a.D + dd) * 4u;
     const Rows<T> ru(a.u, a.u_sb, a.u_st, b), rd(a.delta, a.delta_sb, a.delta_st, b), ro(a.dout, a.dout_sb, a.dout_st, b);
+    const bool gate = a.dz != nullptr;
     const Rows<T> rz(a.z, a.z_sb, a.z_st, b), rb(a.B, a.B_sb, a.B_st, b), rc(a.C, a.C_sb, a.C_st, b);
     const float* kept_b = a.kept + (int64_t)b * ngroup * NT * a.D;
     auto fetch = [&](int t0) {
@@ -827,7 +827,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs a) {
     for (int off = L / 2; off >= 1; off >>= 1) y += __shfl_xor(y, off, 64);
     if (live && n0 == 0) {
         if (a.Dskip) y += a.Dskip[d] * u;
-        if (a.z) {
+        if (a.gate) {
             const float z = elem<T>(a.z, a.z_sb, 0, b, 0, d);
             y *= z * sigmoid_f(z);
         }
@@ -875,6 +875,8 @@ ScanArgs fill(const dpk_scan_desc* s) {
     a.nb = s->B; a.T = s->T; a.D = s->D; a.N = s->N; a.softplus = s->softplus; a.nchunk = s->nchunk; a.chunk = s->chunk;
     const int bl = block_of(s->D);
     a.ndb = (s->D + bl - 1) / bl;
+    a.gate = s->z != nullptr;
+    if (!a.gate) { a.z = a.u; a.z_sb = a.u_sb; a.z_st = a.u_st; }
     a.kept = s->kept; a.edge = s->edge; a.span = s->span;
     return a;
 }
@@ -902,17 +904,18 @@ void join(const ScanArgs& a, hipStream_t st) {
 
 // Chunks of time a scan is cut into.  Cutting costs a second reading of the inputs and most of the arithmetic again, so it has to
 // win a factor of two or three in waves.  Forward into up to 4096 waves (four a SIMD; 1 x 8192 x 1024, N = 16, bf16: 93 us against
-// 100 with 2048) of chunks as short as 32 steps (2 x 4096 x 500: 75 us against 102 with 64), from fewer than 1366 (8 x 1000 x 4096
-// bf16: 323 us against 917 in one piece; 20 x 1000 x 4096: 744 against 918), of short sequences fewer than 512 (50 x 256 x 1024
-// fp32: 134 against 127).  Backward into up to 2048 of at least 64 steps (145 us against 154 with 32: its waves hold 16 channels,
-// so there are four times as many to begin with) from fewer than 512 (8 x 1000 x 4096: 690 us against 643).
+// 100 with 2048) of chunks as short as 32 steps (2 x 4096 x 500: 75 us against 102 with 64), from fewer than 800 (10 x 2000 x 4096
+// bf16, 640 waves: 706 us against 938 in one piece; 16 x 1000 x 4096, 1024 waves: 549 against 491), of short sequences fewer than
+// 512 (50 x 256 x 1024 fp32, 800 waves: 134 against 127).  Backward into up to 2048 of at least 64 steps (145 us against 154 with
+// 32: its waves hold 16 channels, so there are four times as many to begin with) from fewer than 512 (8 x 1000 x 4096: 690 us
+// against 643).
 extern "C" int dpk_selective_scan_chunks(int B, int T, int D, int backward, int* chunk) {
     if (B <= 0 || T <= 0 || D <= 0) {
         if (chunk) *chunk = (T > 0 ? (T + GROUP - 1) / GROUP * GROUP : 0);
         return 1;
     }
     const int64_t waves = (int64_t)B * ((D + 63) / 64);
-    int64_t n = waves >= (backward || T < 512 ? 512 : 1366) ? 1 : (backward ? 2048 : 4096) / waves;
+    int64_t n = waves >= (backward || T < 512 ? 512 : 800) ? 1 : (backward ? 2048 : 4096) / waves;
     const int shortest = backward ? 64 : 32;
     const int64_t most = (T + shortest - 1) / shortest;
     if (n > most) n = most;
@@ -965,7 +968,6 @@ extern "C" int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_sca
     const int blocks = back_blocks_of(s->D, s->N);
     if (blocks > 1 && s->T > 0 && !g->dbc) return DPK_EINVAL;
     a.dout = g->dout; a.dhT = g->dhT; a.du = g->du; a.ddelta = g->ddelta; a.dB = g->dB; a.dC = g->dC; a.dz = s->z ? g->dz : nullptr;
-    if (!a.z) { a.z = a.u; a.z_sb = a.u_sb; a.z_st = a.u_st; }
     a.dh0 = g->dh0; a.dbc = g->dbc; a.dA = g->dA; a.dD = g->dD; a.dbias = g->dbias; a.par_stride = g->par_stride;
     a.dout_sb = g->dout_sb; a.dout_st = g->dout_st; a.scale = g->scale; a.accumulate = g->accumulate;
     const hipStream_t st = (hipStream_t)stream;
