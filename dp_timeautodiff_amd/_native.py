@@ -735,7 +735,9 @@ def _as_btf(t: torch.Tensor):
     """[B, T, F] whose last dimension is contiguous (and whose rows are less than 2^24 elements apart: the scan's lanes count a
     group's rows in 32-bit byte offsets)."""
     s = t.stride()
-    return t if (s[2] == 1 or t.shape[2] == 1) and s[1] < 1 << 24 else t.contiguous()
+    if s[1] >= 1 << 24:  # cloned: of a single step torch calls any distance contiguous
+        return t.clone(memory_format=torch.contiguous_format)
+    return t if s[2] == 1 or t.shape[2] == 1 else t.contiguous()
 
 
 def _sum_rows(device, src: int, groups: int, rows: int, in_stride: int, outs, scale: float, accumulate: bool):

@@ -397,6 +397,24 @@ def test_selective_scan_gradient_against_differences(seed):
         assert abs(slope - want) < 1e-2 * max(abs(want), norm), n
 
 
+def test_single_steps_of_any_row_distance():
+    from dp_timeautodiff_amd.layers import causal_conv, selective_scan
+    args, dout, _, _ = scan_inputs((3, 1, 20, 4, "zdbs", None), torch.float32)
+    args, dout = [None if t is None else t.cuda() for t in args[:8]], dout.cuda()
+
+    def odd(t):   # the same memory: a dimension of one has any distance
+        return t.as_strided(t.shape, (t.stride(0), 2 ** 40, 1)) if t.dim() == 3 else t
+
+    for fn in (lambda *a: selective_scan(*a), lambda u, *_: causal_conv(u, args[7].new_ones(20, 3))):
+        grads = []
+        for view in (lambda t: t, odd):
+            leaves = [None if t is None else view(t).detach().requires_grad_() for t in args]
+            y = fn(*leaves)
+            y.backward(view(dout))
+            grads.append([y.detach()] + [t.grad for t in leaves if t is not None and t.grad is not None])
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
 def test_offsets_past_32_bits():
     """Batch strides of 2^31 + elements: both sequences of a two-sequence view, the second one far out."""
     from dp_timeautodiff_amd.layers import causal_conv, rms_norm, selective_scan
