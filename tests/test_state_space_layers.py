@@ -1,6 +1,6 @@
 """The state-space layers under the DP engine: per-sample gradients, clipping, accumulation, shared layers, 8-bit stash, graphs.
 
-Checker: the same module arithmetic in float64 (tests/state_space_reference.py), one sample at a time, by autograd.  Every test runs
+Oracle: the same module arithmetic in float64 (tests/state_space_reference.py), one sample at a time, by autograd.  Every test runs
 twice: "hip" (gpu: the kernels) and "oracle" (CPU: the same host code on stand-ins of the kernels).  Tolerance: 1e-5 of the
 tensor's largest value, the framework's bar for per-sample gradients."""
 import math
