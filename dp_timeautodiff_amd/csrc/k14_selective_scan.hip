@@ -11,10 +11,10 @@
 // channels, so every access of a wave is one run of memory); B_t and C_t are the same for all channels and are staged in LDS for
 // GROUP steps at a time.
 // The backward pass needs the states in reverse.  Undoing the recurrence would divide by decays near 0, so the forward pass
-// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16; not of the first group where it is 0), and the backward pass recomputes
-// a group's states and decays into registers.  A channel's states lie on LS = N / 4 lanes there, so that three waves a SIMD fit
-// (with all 16 on one lane, one wave a SIMD: 1887 us at 256 x 256 x 1024; with eight, the group spilled and waited for its spills:
-// 3311); what a channel has once per step (softplus, gates, loads, stores) is dealt over those lanes by step, and passed round by
+// keeps the state at the start of every group of 8 steps (8 bytes a channel and step at N = 16; not of the first group where it is
+// 0), and the backward pass recomputes a group's states and decays into registers.  A channel's states lie on LS = N / 4 lanes there,
+// so that three waves a SIMD fit (with all 16 on one lane, one wave a SIMD: 1887 us at 256 x 256 x 1024; with eight, the group spilled
+// and waited for its spills: 3311); what a channel has once per step (softplus, gates, loads, stores) is dealt over those lanes by step, and passed round by
 // lane swaps.
 // Per state and step: forward one v_exp_f32 (quarter rate) and four plain instructions, backward one and twelve, and the sums
 // over channels for dB and dC, a halving tree over the lanes (four more).  Measured at 256 x 256 x 1024, N = 16, fp32: forward
