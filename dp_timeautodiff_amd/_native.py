@@ -787,6 +787,7 @@ def rms_norm_backward(r, residual, dy, dr, weight, rstd, want_dx: bool, want_dw:
     C = r.shape[-1]
     rows = r.numel() // C
     groups = r.shape[0] if window is not None else 1
+    weight = _dense(weight)
     r, ld_r = _as_rows(r)
     dy, ld_dy = _as_rows(dy)
     ld_dr = ld_res = 0

@@ -1,0 +1,91 @@
+"""Calls of the state-space operators at the edges of what they take: layouts of parameters, infinite steps, the types' largest
+values, sizes past what a launch can count, other ways of differentiating.  Oracle and tolerances: those of
+tests/test_state_space_gpu.py (1e-5 of a tensor's largest value, half a step of a 16-bit result)."""
+import ctypes
+
+import pytest
+import torch
+import torch.nn as nn
+
+import state_space_reference as R
+
+F32 = 1e-5
+
+
+# ---- parameters that are not dense ------------------------------------------------------------------------------------------------
+
+
+def test_norm_backward_reads_a_dense_weight(monkeypatch):
+    """What the launch is handed, seen on the host: C floats of the weight's own values, wherever they stood."""
+    from dp_timeautodiff_amd import _native
+    _native.load()
+    seen = {}
+
+    def call(name, device, *args):
+        if name == "dpk_rms_norm_backward":
+            address = args[8]
+            seen["address"] = address
+            if seen.get("read"):
+                seen["weight"] = torch.frombuffer(bytearray(ctypes.string_at(address, 4 * 6)), dtype=torch.float32)
+
+    monkeypatch.setattr(_native, "_call", call)
+    r, dy, rstd = torch.ones(3, 6), torch.ones(3, 6), torch.ones(3)
+    wide = torch.arange(12.0)
+    seen["read"] = True
+    _native.rms_norm_backward(r, None, dy, None, wide[::2], rstd, True, True)
+    assert torch.equal(seen["weight"], wide[::2])
+    one = torch.tensor([3.0])
+    seen["read"] = False   # (of an expanded weight's own storage only the first float may be read)
+    _native.rms_norm_backward(r, None, dy, None, one.expand(6), rstd, True, True)
+    assert seen["address"] != one.data_ptr()
+
+
+def _layouts(dense):
+    """The same values: every second element of a wider tensor, a transposed one, and the tensor itself."""
+    wide = torch.stack([dense, torch.full_like(dense, 7.0)], -1).flatten(-2)
+    yield wide[..., ::2]
+    if dense.dim() == 2:
+        yield dense.t().contiguous().t()
+    yield dense
+
+
+@pytest.mark.gpu
+def test_parameters_of_any_layout_give_the_same_results():
+    from dp_timeautodiff_amd.layers import causal_conv, rms_norm, selective_scan
+    g = torch.Generator().manual_seed(0)
+    B, T, D, N = 3, 9, 40, 6
+    rnd = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    x, res, delta, z, dy = (rnd(B, T, D) for _ in range(5))
+    Bm, Cm = rnd(B, T, N), rnd(B, T, N)
+    calls = [
+        (lambda u, w: rms_norm(u, w, res)[0], [rnd(D)]),
+        (lambda u, w: rms_norm(u, w)[0], [rnd(D)]),
+        (lambda u, w, b: causal_conv(u, w, b), [rnd(D, 4), rnd(D)]),
+        (lambda u, a, d, b, h: selective_scan(u, delta, a, Bm, Cm, d, z, b, state=h), [rnd(D, N), rnd(D), rnd(D), rnd(B, D, N)])]
+    for k, (fn, params) in enumerate(calls):
+        want = None
+        for views in zip(*([p] + [v for v in _layouts(p)] for p in params)):
+            u = x.clone().requires_grad_()
+            leaves = [v.detach().requires_grad_() for v in views]
+            assert all(v.stride() == w.stride() for v, w in zip(views, leaves))
+            y = fn(u, *leaves)
+            y.backward(dy)
+            got = [y.detach(), u.grad] + [t.grad for t in leaves]
+            want = got if want is None else want
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+    # one number for all channels
+    one = torch.tensor([1.5], device="cuda", requires_grad=True)
+    u = x.clone().requires_grad_()
+    rms_norm(u, one.expand(D), res)[0].backward(dy)
+    u64, one64 = x.cpu().double().requires_grad_(), torch.tensor([1.5], dtype=torch.float64, requires_grad=True)
+    (R.rms_norm(u64, one64.expand(D), res.cpu().double())[0] * dy.cpu().double()).sum().backward()
+    assert float((u.grad.cpu().double() - u64.grad).abs().max()) <= F32 * float(u64.grad.abs().max())
+    # its gradient is a sum of D channels' gradients, each within F32 of the largest
+    dw = rms_grad_terms(x, res, dy)
+    assert float((one.grad.cpu().double() - one64.grad).abs().max()) <= F32 * D * float(dw.abs().max())
+
+
+def rms_grad_terms(x, res, dy):
+    w = torch.full((x.shape[-1],), 1.5, dtype=torch.float64, requires_grad=True)
+    (R.rms_norm(x.cpu().double(), w, res.cpu().double())[0] * dy.cpu().double()).sum().backward()
+    return w.grad
