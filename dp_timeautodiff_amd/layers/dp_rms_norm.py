@@ -9,6 +9,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _native
@@ -59,9 +60,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     Returns (y, r) with r = x + residual (x itself without a residual), or (y, r, Activation8) with `quantize`: y also in 8
     bits, as compress_activation would hold it, without reading y again.  The 8-bit form takes no part in autograd."""
     sink, anchor = _sink if _sink is not None else (None, None)
-    grad = torch.is_grad_enabled() and (anchor is not None or any(
-        isinstance(t, torch.Tensor) and t.requires_grad for t in (x, residual, weight)))
-    if grad:
+    if _wants_autograd(anchor, x, residual, weight):
         out = _RMSNorm.apply(x, residual, weight, eps, quantize, sink, anchor)
     else:
         y, r, _, q, e = _native.rms_norm_forward(x, residual, weight, eps, False, quantize)
@@ -107,6 +106,20 @@ class DPRMSNorm(nn.Module):
             out = (*back, *(Activation8(a.data.transpose(0, 1).contiguous(), a.exponent.transpose(0, 1).contiguous(), a.dtype)
                             for a in out[2:]))
         return out
+
+
+def _wants_autograd(anchor, *tensors) -> bool:
+    """Whether a call has to go through its autograd function: gradients are recorded, or an input carries a forward-mode tangent,
+    for which the function raises (it has no jvp; without it the tangent would be lost and read as zero)."""
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
+    if _has_tangent(*tensors):
+        return True
+    return torch.is_grad_enabled() and (anchor is not None or any(t.requires_grad for t in tensors))
+
+
+def _has_tangent(*tensors) -> bool:
+    return forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _active_claim(module):

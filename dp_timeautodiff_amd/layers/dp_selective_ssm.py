@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _native
 from .dp_rnn import RNNLinear
-from .dp_rms_norm import DPRMSNorm, _active_claim, _copy_without_runtime
+from .dp_rms_norm import DPRMSNorm, _active_claim, _copy_without_runtime, _has_tangent, _wants_autograd
 
 _ACTIVATIONS = {None: False, "silu": True}
 
@@ -29,8 +29,9 @@ def _silu(activation) -> bool:
     return _ACTIVATIONS[activation]
 
 
-def _wants_grad(anchor, *tensors) -> bool:
-    return torch.is_grad_enabled() and (anchor is not None or any(t is not None and t.requires_grad for t in tensors))
+def _refuse_tangents(name: str, *tensors):
+    if _has_tangent(*tensors):
+        raise NotImplementedError(f"{name} is not differentiable: an input carries a forward-mode tangent")
 
 
 class _CausalConv(torch.autograd.Function):
@@ -67,7 +68,7 @@ def causal_conv(x, weight, bias=None, *, activation: Optional[str] = "silu", sta
     [B,W-1,D] holds the rows before the first (zeros if None).  Returns y, or (y, state behind the sequences)."""
     sink, anchor = _sink if _sink is not None else (None, None)
     silu = _silu(activation)
-    if _wants_grad(anchor, x, weight, bias, state):
+    if _wants_autograd(anchor, x, weight, bias, state):
         return _CausalConv.apply(x, weight, bias, state, lengths, silu, return_state, sink, anchor)
     y, out = _native.causal_conv_forward(x, weight, bias, state, lengths, silu, return_state)
     return (y, out) if return_state else y
@@ -75,6 +76,7 @@ def causal_conv(x, weight, bias=None, *, activation: Optional[str] = "silu", sta
 
 def causal_conv_step(x, state, weight, bias=None, *, activation: Optional[str] = "silu"):
     """One token: x [B,D]; `state` [B,W-1,D] is updated in place.  Not differentiable."""
+    _refuse_tangents("causal_conv_step", x, state, weight, bias)
     return _native.causal_conv_step(x, state, weight, bias, _silu(activation))
 
 
@@ -116,7 +118,7 @@ def selective_scan(u, delta, A_log, B, C, D=None, z=None, dt_bias=None, *, softp
     """u, delta, z [B,T,D]; B, C [B,T,N]; A_log [D,N] (N up to 32), D, dt_bias [D], state [B,D,N] fp32.  D, z, dt_bias and
     state may be None (no skip, no gate, no bias, zeros).  Returns out [B,T,D], or (out, final state [B,D,N])."""
     sink, anchor = _sink if _sink is not None else (None, None)
-    if _wants_grad(anchor, u, delta, A_log, B, C, D, z, dt_bias, state):
+    if _wants_autograd(anchor, u, delta, A_log, B, C, D, z, dt_bias, state):
         return _SelectiveScan.apply(u, delta, A_log, B, C, D, z, dt_bias, state, lengths, softplus, return_state, sink, anchor)
     inp = _native.ScanInputs(u, delta, A_log, B, C, D, z, dt_bias, state, lengths, softplus)
     out, hT, _ = _native.selective_scan_forward(inp, False, return_state)
@@ -125,6 +127,7 @@ def selective_scan(u, delta, A_log, B, C, D=None, z=None, dt_bias=None, *, softp
 
 def selective_scan_step(u, delta, A_log, B, C, state, D=None, z=None, dt_bias=None, *, softplus: bool = True):
     """One token: u, delta, z [B,D], B, C [B,N]; `state` [B,D,N] is updated in place.  Not differentiable."""
+    _refuse_tangents("selective_scan_step", u, delta, A_log, B, C, state, D, z, dt_bias)
     return _native.selective_scan_step(_native.ScanInputs(u, delta, A_log, B, C, D, z, dt_bias, None, None, softplus, step=True),
                                        state)
 

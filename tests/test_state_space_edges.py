@@ -89,3 +89,36 @@ def rms_grad_terms(x, res, dy):
     w = torch.full((x.shape[-1],), 1.5, dtype=torch.float64, requires_grad=True)
     (R.rms_norm(x.cpu().double(), w, res.cpu().double())[0] * dy.cpu().double()).sum().backward()
     return w.grad
+
+
+# ---- forward-mode derivatives ------------------------------------------------------------------------------------------------------
+
+
+@pytest.fixture(params=[pytest.param("hip", marks=pytest.mark.gpu), "oracle"])
+def dev(request, monkeypatch):
+    if request.param == "hip":
+        assert torch.cuda.is_available()
+        from dp_timeautodiff_amd import _native
+        _native.load()
+        return torch.device("cuda:0")
+    R.install(monkeypatch)
+    return torch.device("cpu")
+
+
+@pytest.mark.parametrize("record", [True, False])
+def test_a_forward_mode_tangent_is_refused_and_not_dropped(dev, record):
+    from torch.autograd import forward_ad
+    from dp_timeautodiff_amd.layers import causal_conv, causal_conv_step, rms_norm, selective_scan, selective_scan_step
+    t = lambda *s: torch.ones(*s, device=dev)  # noqa: E731
+    x, w, cw, a, b = t(2, 3, 4), t(4), t(4, 2), t(4, 5), t(2, 3, 5)
+    calls = [(rms_norm, [x, w]), (rms_norm, [x, w, x]), (causal_conv, [x, cw]), (causal_conv, [x, cw, w]),
+             (selective_scan, [x, x, a, b, b]), (selective_scan, [x, x, a, b, b, w, x, w]),
+             (causal_conv_step, [t(2, 4), t(2, 1, 4), cw, w]),
+             (selective_scan_step, [t(2, 4), t(2, 4), a, t(2, 5), t(2, 5), t(2, 4, 5), w, t(2, 4), w])]
+    with torch.set_grad_enabled(record), forward_ad.dual_level():
+        for fn, args in calls:
+            for k, arg in enumerate(args):
+                dual = forward_ad.make_dual(arg, torch.ones_like(arg))
+                with pytest.raises(NotImplementedError):
+                    fn(*[dual if i == k else v for i, v in enumerate(args)])
+        rms_norm(x, w)   # a level without a tangent is of no account
