@@ -4,7 +4,9 @@ A DP-SGD step keeps the input of every Linear until the backward pass contracts 
 stash is what bounds the physical batch of long sequences after the per-sample-gradient arena.  `compress_activation` keeps a
 tensor as one signed byte per element and one exponent byte per 128 neighbours of the last dimension (the scale is a
 power of two, so the stored value is the correctly rounded quotient); `restore_activation` gives back the values the bytes
-stand for.  The error of an element is at most max|block| / 127.  A block that holds an inf or NaN restores as NaN.
+stand for.  The error of an element is at most max|block| / 127 (in a block whose values are under 2^-120, at most 2^-127; in one
+with a value from 127 * 2^121 on, at most 2^122).  No finite value restores as inf in the dtype it had.  A block that holds an inf
+or NaN restores as NaN.
 
 `GradSampleModule(..., activation_bits=8)` stashes Linear inputs this way.  Clipping bounds whatever gradient comes out, so the
 privacy guarantee is untouched; the gradients carry the rounding of the activations.

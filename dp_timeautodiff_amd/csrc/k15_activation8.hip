@@ -4,8 +4,10 @@
 // A block of 128 neighbours of a row shares one scale 2^k, k the least integer with max|v| <= 127 * 2^k; an element is kept as
 // q = rint(v * 2^-k).  The scale being a power of two, v * 2^-k is exact, so q is the correctly rounded quotient, the error
 // is at most 2^k / 2 <= max|v| / 127, and q * 2^k is exact in bf16 too.  (A scale of max/127 would halve the worst error but
-// make q depend on the last bit of a division.)  Blocks that hold an inf or NaN restore as NaN: an overflow in the forward pass
-// stays visible in the gradients.
+// make q depend on the last bit of a division.)  The error is larger than max|v| / 127 in two places: under the least scale, 2^-126,
+// where it is up to 2^-127, and at k = 122, where q is held to 63 (64 * 2^122 is no fp32 number) and it is up to 2^122.  What rounds
+// up to 2^16 (fp16 from 65024 on: q = 64, k = 10) is restored in fp16 as its largest value, 65504, and not as inf.  Blocks that hold
+// an inf or NaN restore as NaN: an overflow in the forward pass stays visible in the gradients.
 // Both directions are HBM-bound: 4 + 1 + 1/128 bytes an fp32 element.  Lanes take 16 bytes of the wide side each (32 lanes a block in
 // fp32, 16 in 16 bits), so that every access of a wave is one run of memory, and a workgroup has four or two rounds of blocks
 // under way.
@@ -136,7 +138,11 @@ __global__ void __launch_bounds__(256) restore_kernel(const int8_t* __restrict__
         const float s = exponent_value(eb[k]);
         float v[LV];
 #pragma unroll
-        for (int i = 0; i < LV; ++i) v[i] = (float)(int8_t)(w[k][i / 4] >> (8 * (i % 4))) * s;
+        for (int i = 0; i < LV; ++i) {
+            v[i] = (float)(int8_t)(w[k][i / 4] >> (8 * (i % 4))) * s;
+            if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16))
+                v[i] = fabsf(v[i]) == 65536.f ? __builtin_copysignf(65504.f, v[i]) : v[i];
+        }
         if (u.n > 0) store_n<T, LV>(X + u.row * C + u.c, u.n, v);
     }
 }

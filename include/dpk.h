@@ -410,8 +410,10 @@ int dpk_selective_scan_step(const dpk_scan_desc* s, float* state, void* out, voi
 
 /*
  * K15: X [rows, C] (row stride ld_x) as Q int8 [rows, C] and one exponent byte per block of 128 elements of a row, QE [rows,
- * ceil(C/128)]: with k the least integer >= -126 such that max|x| <= 127 * 2^k, q = rint(x * 2^-k) and the byte is k + 127 (at k = 122 |q| is
- * held to 63, so that no finite value restores as inf).  A block that holds an inf or NaN has the byte 255 and restores as NaN.  restore writes q * 2^k in any dtype.
+ * ceil(C/128)]: with k the least integer >= -126 such that max|x| <= 127 * 2^k, q = rint(x * 2^-k) and the byte is k + 127.  No finite value
+ * restores as inf in its own dtype: at k = 122 |q| is held to 63, and 2^16 is written as 65504 in fp16.  The error is at most max|block| / 127,
+ * at k = 122 at most 2^122, and 2^-127 where the block's values are smaller still.  A block that holds an inf or NaN has the byte 255
+ * and restores as NaN.  restore writes q * 2^k in any dtype.
  * dpk_sum_rows: scale * sum_r in[g][r][c] in a fixed order, rows of in_stride floats; the first n[0] columns go (or are added) to
  * out[0] + g * out_stride[0], the next n[1] to out[1], the next n[2] to out[2] (host arrays of three; n = 0: none).  Joins the
  * partial parameter gradients of K12..K14.

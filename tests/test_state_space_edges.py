@@ -122,3 +122,43 @@ def test_a_forward_mode_tangent_is_refused_and_not_dropped(dev, record):
                 with pytest.raises(NotImplementedError):
                     fn(*[dual if i == k else v for i, v in enumerate(args)])
         rms_norm(x, w)   # a level without a tangent is of no account
+
+
+# ---- 8 bits at the ends of a type's range ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_finite_fp16_values_restore_as_finite():
+    """65056 is 63.53 * 2^10: it is held as 64 * 2^10 = 2^16, which fp16 has no number for.  Off by at most max / 127 all the same."""
+    from dp_timeautodiff_amd.activation8 import compress_activation, restore_activation
+    for top in (65024.0, 65056.0, 65504.0):
+        for C in (1, 5, 128, 260):
+            x = torch.linspace(-1.0, 1.0, 2 * C).reshape(2, C)
+            x[0, 0], x[1, C // 2] = top, -top
+            x[0, C - 1] = 65024.0   # just on the border of q = 63 and 64 where the block has a larger value
+            x = x.to(torch.float16)
+            a = compress_activation(x.cuda())
+            q, e = R.compress(x)
+            assert torch.equal(a.data.cpu(), q) and torch.equal(a.exponent.cpu(), e)
+            back = restore_activation(a).cpu().double()
+            assert torch.equal(back, R.restore(q, e).clamp(-65504, 65504).to(torch.float16).double())
+            assert bool(torch.isfinite(back).all())
+            most = torch.nn.functional.pad(x.double().abs(), (0, -C % 128)).unflatten(-1, (-1, 128)).amax(-1)
+            assert bool(((back - x.double()).abs() <= most.repeat_interleave(128, -1)[..., :C] / 127).all())
+            assert torch.equal(restore_activation(a, torch.float32).cpu().double(), R.restore(q, e))
+    # what fp16 never held goes by fp16's own rounding
+    a = compress_activation(torch.tensor([[131072.0, -1.0]], device="cuda"))
+    assert restore_activation(a, torch.float16)[0, 0].isinf() and torch.isfinite(restore_activation(a)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_errors_at_both_ends_of_the_scales(dev, dtype):
+    """At k = 122, q is held to 63 and an element is off by at most 2^122; under the least scale by at most 2^-127."""
+    from dp_timeautodiff_amd.activation8 import compress_activation, restore_activation
+    big = torch.full((1, 128), torch.finfo(dtype).max, dtype=dtype)
+    big[0, 1:64] = -torch.rand(63, generator=torch.Generator().manual_seed(0)).to(dtype) * torch.finfo(dtype).max
+    small = torch.linspace(-2.0 ** -125, 2.0 ** -125, 128).reshape(1, 128).to(dtype)
+    for x, most in ((big, 2.0 ** 122), (small, 2.0 ** -127)):
+        back = restore_activation(compress_activation(x.to(dev)))
+        assert back.dtype == dtype and bool(torch.isfinite(back).all())
+        assert float((back.cpu().double() - x.double()).abs().max()) <= most
