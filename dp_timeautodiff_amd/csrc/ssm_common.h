@@ -72,13 +72,14 @@ __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rc
 
 // log(1 + e^x) and its derivative, the sigmoid.  e^x = 2^(x log2 e): the product's rounding error, times ln 2, is put back as a
 // factor, so e keeps its relative accuracy for x << 0.  With w = fl(1 + e) the logarithm of w misses log(1 + e) by the rounding
-// of w; the factor e / (w - 1) puts that back (w - 1 is exact).  Above 20 the result is x to the last bit of fp32.
+// of w; the factor e / (w - 1) puts that back (w - 1 is exact).  Above 20 the result is x to the last bit of fp32.  Below -150 e^x is
+// 0; x is held there, since the product's rounding error is inf - inf from -2.4e38 on.
 struct Softplus {
     float value, slope;
 };
 __device__ __forceinline__ Softplus softplus_f(float x) {
     constexpr float LOG2E_LOW = 1.9259629911266175e-8f;   // log2 e = LOG2E + LOG2E_LOW
-    const float xc = x < 20.f ? x : 20.f;
+    const float xc = __builtin_amdgcn_fmed3f(x, -150.f, 20.f);
     const float p = xc * LOG2E;
     const float low = __builtin_fmaf(xc, LOG2E, -p) + xc * LOG2E_LOW;
     const float e0 = exp2_hw(p);

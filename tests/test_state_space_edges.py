@@ -162,3 +162,58 @@ def test_errors_at_both_ends_of_the_scales(dev, dtype):
         back = restore_activation(compress_activation(x.to(dev)))
         assert back.dtype == dtype and bool(torch.isfinite(back).all())
         assert float((back.cpu().double() - x.double()).abs().max()) <= most
+
+
+# ---- steps of size 0 by an infinite delta ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_softplus_at_the_ends_of_the_range():
+    """Below -87 e^x leaves fp32's normal numbers and may come out as 0: 2^-126 of allowance there."""
+    from dp_timeautodiff_amd.layers import selective_scan
+    x = torch.tensor([-float("inf"), -3.4e38, -2.5e38, -1e30, -1e4, -151.0, -150.0, -149.0, -104.0, -90.0, -87.0, -20.0, 0.0, 19.999, 20.0, 20.001,
+                      88.0, 1e4])
+    d = x.numel()
+    one = torch.ones(1, 1, 1)
+    delta = x.view(1, 1, d).cuda().requires_grad_()
+    _, h = selective_scan(torch.ones(1, 1, d).cuda(), delta, torch.zeros(d, 1).cuda(), one.cuda(), one.cuda(), return_state=True)
+    ref = torch.logaddexp(x.double(), torch.zeros((), dtype=torch.float64))
+    off = (h.detach().view(d).double().cpu() - ref).abs()
+    assert bool((off <= 16 * 2.0 ** -24 * ref + 2.0 ** -126).all())
+    h.sum().backward()
+    assert bool(((delta.grad.view(d).double().cpu() - torch.sigmoid(x.double())).abs() <= F32 * torch.sigmoid(x.double()) + 2.0 ** -126).all())
+    for bad, seen in ((float("inf"), torch.isinf), (float("nan"), torch.isnan)):
+        _, h = selective_scan(one.cuda(), torch.full((1, 1, 1), bad).cuda(), torch.zeros(1, 1).cuda(), one.cuda(), one.cuda(), return_state=True)
+        assert bool(seen(h).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", [(3, 20, 70, 16, "zdbsh", None), (1, 700, 40, 16, "zdsh", [611]), (2, 9, 65, 4, "zdbs", [9, 3])], ids=str)
+def test_steps_masked_by_an_infinite_delta_leave_the_state(dtype, case):
+    import test_state_space_gpu as G
+    from dp_timeautodiff_amd.layers import selective_scan, selective_scan_step
+    args, dout, dh, lengths = G.scan_inputs(case, dtype)
+    args[1][:, ::3] = -float("inf")
+    args[1][0, 1, 0] = -float("inf")
+    l64 = G.leaf64(*args)
+    o_ref, h_ref = R.selective_scan(*l64[:8], state=l64[8], lengths=lengths)
+    lg = G.leaf(*args)
+    out, h = selective_scan(*lg[:8], state=lg[8], lengths=None if lengths is None else lengths.cuda(), return_state=True)
+    G.close(out, o_ref, "out")
+    G.close(h, h_ref, "state")
+    ((o_ref * dout.double()).sum() + (h_ref * dh.double()).sum()).backward()
+    torch.autograd.backward((out, h), (dout.cuda(), dh.cuda()))
+    for n, a, b in zip(G.NAMES, lg, l64):
+        if a is not None:
+            assert bool(torch.isfinite(b.grad).all()), n
+            extra = 0.0
+            if n == "u":   # two terms that may cancel: 1e-5 of each
+                skip = (dout.double() * (1.0 if args[6] is None else torch.nn.functional.silu(args[6].double())) * args[5].double()).abs()
+                extra = F32 * (2 * skip + b.grad.abs())
+            G.close(a.grad, b.grad, "d" + n, extra)
+    state = torch.randn(2, 5, 3, device="cuda")
+    kept = state.clone()
+    y = selective_scan_step(torch.ones(2, 5, device="cuda"), torch.full((2, 5), -float("inf"), device="cuda"), torch.zeros(5, 3, device="cuda"),
+                            torch.ones(2, 3, device="cuda"), torch.ones(2, 3, device="cuda"), state)
+    assert torch.equal(state, kept) and bool(torch.isfinite(y).all())
