@@ -995,7 +995,8 @@ def selective_scan_forward(inp: ScanInputs, want_kept: bool, want_state: bool):
     out = u.new_empty((b, t, d))
     hT = torch.empty(b, d, n, dtype=torch.float32, device=u.device) if want_state else None
     g = lib.dpk_selective_scan_group()
-    kept = torch.empty(b, max((t + g - 1) // g - (inp.h0 is None), 1), lib.dpk_selective_scan_state_rows(n), d, dtype=torch.float32,
+    groups = max((t + g - 1) // g - (inp.h0 is None), 0)   # with a kept state; where there are none, one group's room for all
+    kept = torch.empty(b if groups else min(b, 1), max(groups, 1), lib.dpk_selective_scan_state_rows(n), d, dtype=torch.float32,
                        device=u.device) if want_kept else None
     if b:
         s, scratch = inp.desc(kept)

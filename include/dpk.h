@@ -374,7 +374,7 @@ int dpk_causal_conv_step(const void* x, int64_t x_sb, void* state, const float* 
  * y = Cm_t . h_t + Dskip u_t, out = y silu(z).  u, delta, z [B,T,D], Bm, Cm [B,T,N], N <= DPK_SCAN_MAX_STATE; Dskip, z, dt_bias, h0
  * [B,D,N], lengths [B] may be NULL.  Rows are less than 2^24 elements apart.  Rows at and behind lengths[b] leave the state alone and give out = 0.
  * kept: [B, G, dpk_selective_scan_state_rows(N), D] floats, written by forward where the backward pass is to follow (else NULL); G =
- * ceil(T / dpk_selective_scan_group()), without h0 one less, but at least 1.
+ * ceil(T / dpk_selective_scan_group()), without h0 one less; where G is 0, [1, 1, dpk_selective_scan_state_rows(N), D] floats that are not written.
  * nchunk, chunk: as dpk_selective_scan_chunks says (or 1 and T rounded up to the group); nchunk > 1 needs edge
  * [nchunk, B, N, D] and span [nchunk, B, D] floats of scratch, not kept between the calls.
  * backward: gradients of every input; dhT (nullable) is the gradient of the final state, dh0 (nullable) receives that of h0.

@@ -217,3 +217,37 @@ def test_steps_masked_by_an_infinite_delta_leave_the_state(dtype, case):
     y = selective_scan_step(torch.ones(2, 5, device="cuda"), torch.full((2, 5), -float("inf"), device="cuda"), torch.zeros(5, 3, device="cuda"),
                             torch.ones(2, 3, device="cuda"), torch.ones(2, 3, device="cuda"), state)
     assert torch.equal(state, kept) and bool(torch.isfinite(y).all())
+
+
+# ---- states kept for the backward pass ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("T,carried,groups", [(0, False, 0), (1, False, 0), (8, False, 0), (9, False, 1), (17, False, 2), (0, True, 0), (1, True, 1),
+                                              (8, True, 1), (9, True, 2)])
+def test_no_memory_is_held_for_groups_without_a_kept_state(monkeypatch, T, carried, groups):
+    from dp_timeautodiff_amd import _native
+    _native.load()
+    monkeypatch.setattr(_native, "_call", lambda *a: None)
+    B, D, N = 6, 10, 5
+    u, bc = torch.zeros(B, T, D), torch.zeros(B, T, N)
+    inp = _native.ScanInputs.checked(u, u, torch.zeros(D, N), bc, bc, None, None, None, torch.zeros(B, D, N) if carried else None, None, True)
+    _, _, kept = _native.selective_scan_forward(inp, True, False)
+    assert kept.numel() == (B * groups if groups else 1) * 8 * D   # N = 5 takes 8 rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 7, 8, 9])
+def test_many_short_sequences(T):
+    import test_state_space_gpu as G
+    from dp_timeautodiff_amd.layers import selective_scan
+    args, dout, _, _ = G.scan_inputs((130, T, 70, 6, "zdbs", None), torch.float32)
+    l64, lg = G.leaf64(*args), G.leaf(*args)
+    ref, _ = R.selective_scan(*l64[:8])
+    (ref * dout.double()).sum().backward()
+    selective_scan(*lg[:8]).backward(dout.cuda())
+    for n, a, b in zip(G.NAMES[:8], lg, l64):
+        extra = 0.0
+        if n == "u":   # two terms that may cancel: 1e-5 of each
+            skip = (dout.double() * torch.nn.functional.silu(args[6].double()) * args[5].double()).abs()
+            extra = F32 * (2 * skip + b.grad.abs())
+        G.close(a.grad, b.grad, "d" + n, extra)
