@@ -253,6 +253,10 @@ class _Claim:
         # stream of that graph
         return torch.empty((), device=self._layer.params[0].device, requires_grad=True)
 
+    def parameter(self, p):
+        """The parameter as the layer's autograd function is to see it: detached where nobody reads the summed gradient."""
+        return p.detach() if self._gsm.skip_autograd_param_grads else p
+
     @property
     def batch_first(self):
         return self._gsm.batch_first

@@ -18,7 +18,7 @@ from ..activation8 import Activation8
 
 class _RMSNorm(torch.autograd.Function):
     """(x, residual, weight) -> y, r (r only with a residual), q, e (only with `quantize`).  `sink`: the per-sample gradients'
-    destination, with the weight passed detached; `anchor` keeps the node in the graph when x is data."""
+    destination, with the weight passed detached (unless the engine wants the summed gradients as well); `anchor` keeps the node in the graph when x is data."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps, quantize, sink, anchor):
@@ -47,7 +47,8 @@ class _RMSNorm(torch.autograd.Function):
             with ctx.sink(r.shape[0]) as to:
                 dx, _ = _native.rms_norm_backward(r, residual, dy, dr, weight, rstd, need_x or need_res, True, to.window("weight"),
                                                   to.scale, to.accumulate)
-            dw = None
+            # the summed gradient too, where the engine was asked to leave it to autograd
+            dw = _native.rms_norm_backward(r, residual, dy, None, weight, rstd, False, True)[1] if need_w else None
         else:
             dx, dw = _native.rms_norm_backward(r, residual, dy, dr, weight, rstd, need_x or need_res, need_w)
         return dx if need_x else None, dx if need_res else None, dw, None, None, None, None
@@ -100,7 +101,7 @@ class DPRMSNorm(nn.Module):
         swap = not claim.batch_first and not self.batch_major and x.dim() >= 3  # samples along dimension 1: the kernel wants a sample's rows together
         if swap:
             x, residual = (None if t is None else t.transpose(0, 1).contiguous() for t in (x, residual))
-        out = rms_norm(x, self.weight.detach(), residual, eps=self.eps, quantize=quantize, _sink=(claim.sink, claim.anchor))
+        out = rms_norm(x, claim.parameter(self.weight), residual, eps=self.eps, quantize=quantize, _sink=(claim.sink, claim.anchor))
         if swap:
             back = [t.transpose(0, 1) for t in out[:2]]
             out = (*back, *(Activation8(a.data.transpose(0, 1).contiguous(), a.exponent.transpose(0, 1).contiguous(), a.dtype)

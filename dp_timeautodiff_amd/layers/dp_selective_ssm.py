@@ -55,10 +55,11 @@ class _CausalConv(torch.autograd.Function):
             with ctx.sink(x.shape[0]) as to:
                 wins = (to.window("weight"), to.window("bias") if bias is not None else None)
                 dx, ds, _ = _native.causal_conv_backward(*args, True, wins, to.scale, to.accumulate)
-            dw = db = None
+            # the summed gradients too, where the engine was asked to leave them to autograd
+            grads = _native.causal_conv_backward(*args, True)[2] if need_w or need_b else None
         else:
             dx, ds, grads = _native.causal_conv_backward(*args, need_w or need_b)
-            dw, db = grads if grads is not None else (None, None)
+        dw, db = grads if grads is not None else (None, None)
         return dx if need_x else None, dw, db, ds, None, None, None, None, None
 
 
@@ -96,6 +97,7 @@ class _SelectiveScan(torch.autograd.Function):
         *operands, kept = ctx.saved_tensors
         inp = _native.ScanInputs.checked(*operands, ctx.softplus)
         need = ctx.needs_input_grad
+        need_par = need[2] or need[5] or need[7]
         if dout is None:
             dout = torch.zeros_like(inp.u)
         if ctx.sink is not None:
@@ -104,11 +106,11 @@ class _SelectiveScan(torch.autograd.Function):
                                               for n, t in (("D", inp.D), ("dt_bias", inp.dt_bias))))
                 du, ddelta, dB, dC, dz, dh0, _ = _native.selective_scan_backward(inp, kept, dout, dstate, need[8], True, wins,
                                                                                  to.scale, to.accumulate)
-            grads = (None, None, None)
+            # the summed gradients too, where the engine was asked to leave them to autograd
+            grads = _native.selective_scan_backward(inp, kept, dout, dstate, False, True)[6] if need_par else None
         else:
-            du, ddelta, dB, dC, dz, dh0, grads = _native.selective_scan_backward(inp, kept, dout, dstate, need[8],
-                                                                                 need[2] or need[5] or need[7])
-            grads = grads if grads is not None else (None, None, None)
+            du, ddelta, dB, dC, dz, dh0, grads = _native.selective_scan_backward(inp, kept, dout, dstate, need[8], need_par)
+        grads = grads if grads is not None else (None, None, None)
         out = (du, ddelta, grads[0], dB, dC, grads[1], dz, grads[2], dh0)
         return (*(g if n else None for g, n in zip(out, need)), None, None, None, None, None)
 
@@ -156,7 +158,7 @@ class DPCausalConv(nn.Module):
         claim = _active_claim(self)
         w, b, sink = self.weight, self.bias, None
         if claim is not None:
-            w, b, sink = w.detach(), None if b is None else b.detach(), (claim.sink, claim.anchor)
+            w, b, sink = claim.parameter(w), None if b is None else claim.parameter(b), (claim.sink, claim.anchor)
         return causal_conv(x, w, b, activation=self.activation, state=state, lengths=lengths, return_state=return_state, _sink=sink)
 
     def step(self, x, state):
@@ -190,7 +192,7 @@ class DPSelectiveScan(nn.Module):
         claim = _active_claim(self)
         par, sink = (self.A_log, self.D, self.dt_bias), None
         if claim is not None:
-            par, sink = tuple(p.detach() for p in par), (claim.sink, claim.anchor)
+            par, sink = tuple(claim.parameter(p) for p in par), (claim.sink, claim.anchor)
         return selective_scan(u, delta, par[0], B, C, par[1], z, par[2], state=state, lengths=lengths, return_state=return_state,
                               _sink=sink)
 

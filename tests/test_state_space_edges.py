@@ -251,3 +251,29 @@ def test_many_short_sequences(T):
             skip = (dout.double() * torch.nn.functional.silu(args[6].double()) * args[5].double()).abs()
             extra = F32 * (2 * skip + b.grad.abs())
         G.close(a.grad, b.grad, "d" + n, extra)
+
+
+# ---- under the engine -----------------------------------------------------------------------------------------------------------------
+
+
+def _engine_net(dev, B=4, T=6, **kw):
+    import test_state_space_layers as L
+    net = L.make_net(dev, **kw)
+    x, w = L.data(B, T)
+    return net, x, w, L.reference(net, x, w), L.check
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_summed_gradients_are_left_to_autograd_when_asked(dev, shared):
+    """skip_autograd_param_grads=False: p.grad beside p.grad_sample, for these layers as for Linear ones."""
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    net, x, w, want, check = _engine_net(dev, shared=shared)
+    gsm = GradSampleModule(net, loss_reduction="sum", skip_autograd_param_grads=False)
+    (gsm(x.to(dev)) * w.to(dev)).sum().backward()
+    gsm.check_complete()
+    check(net, want)
+    for n, p in net.named_parameters():
+        total = want[n].sum(0)
+        # each sample's gradient is within F32 of the largest, so their sum is within B times that
+        assert p.grad is not None, n
+        assert float((p.grad.cpu().double() - total).abs().max()) <= F32 * x.shape[0] * float(want[n].abs().max()), n
