@@ -443,6 +443,9 @@ class GradSampleModule(nn.Module):
         for h in self._handles:
             h.remove()
         self._handles = []
+        for sub in self._module.modules():
+            if "_dpk_claim" in sub.__dict__:
+                object.__setattr__(sub, "_dpk_claim", None)
 
     def disable_hooks(self):
         self.hooks_enabled = False
@@ -453,8 +456,6 @@ class GradSampleModule(nn.Module):
     def _close(self):
         self.remove_hooks()
         for sub in self._module.modules():
-            if "_dpk_claim" in sub.__dict__:
-                object.__setattr__(sub, "_dpk_claim", None)
             if "_dpk_sink" in sub.__dict__:
                 object.__setattr__(sub, "_dpk_sink", None)
                 object.__setattr__(sub, "_dpk_sink_active", None)

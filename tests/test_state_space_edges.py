@@ -277,3 +277,14 @@ def test_summed_gradients_are_left_to_autograd_when_asked(dev, shared):
         # each sample's gradient is within F32 of the largest, so their sum is within B times that
         assert p.grad is not None, n
         assert float((p.grad.cpu().double() - total).abs().max()) <= F32 * x.shape[0] * float(want[n].abs().max()), n
+
+
+def test_removed_hooks_leave_all_layers_to_autograd(dev):
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    net, x, w, want, _ = _engine_net(dev)
+    gsm = GradSampleModule(net)
+    gsm.remove_hooks()
+    (gsm(x.to(dev)) * w.to(dev)).sum().backward()
+    for n, p in net.named_parameters():
+        assert p.grad_sample is None and p.grad is not None, n
+        assert float((p.grad.cpu().double() - want[n].sum(0)).abs().max()) <= F32 * x.shape[0] * float(want[n].abs().max()), n
