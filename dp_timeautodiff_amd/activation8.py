@@ -34,3 +34,9 @@ def compress_activation(x: torch.Tensor) -> Activation8:
 def restore_activation(a: Activation8, dtype: torch.dtype = None) -> torch.Tensor:
     """The values `a` stands for, in the compressed tensor's dtype or in `dtype`."""
     return _native.restore_activation(a.data, a.exponent, a.dtype if dtype is None else dtype)
+
+
+def belongs_to(a: Activation8, x: torch.Tensor) -> bool:
+    """Whether `a` can be `x` in 8 bits: its shape, dtype and device.  (Not whether it holds x's values.)"""
+    return (isinstance(a, Activation8) and a.dtype == x.dtype and a.data.device == x.device == a.exponent.device
+            and a.data.shape == x.shape and a.exponent.shape == x.shape[:-1] + (-(-x.shape[-1] // _native.ACT8_BLOCK),))

@@ -29,7 +29,7 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .activation8 import Activation8, compress_activation, restore_activation
+from .activation8 import Activation8, belongs_to, compress_activation, restore_activation
 from .layers import DPCausalConv, DPRMSNorm, DPSelectiveScan, RNNLinear, SequenceBias, SSMLinear
 from .layers.fused_gru import FusedLinearCellGRU
 
@@ -508,7 +508,10 @@ class GradSampleModule(nn.Module):
                 return tapped
             if self.activation_bits == 8 and layer.kind == "linear":
                 kept = inputs[1] if len(inputs) > 1 else None
-                layer.acts.append(kept if isinstance(kept, Activation8) else compress_activation(inputs[0]))
+                if kept is not None and not belongs_to(kept, inputs[0]):
+                    raise ValueError(f"{layer.name}: what was passed as the input in 8 bits does not belong to the input "
+                                     f"({tuple(inputs[0].shape)}, {inputs[0].dtype}, {inputs[0].device})")
+                layer.acts.append(compress_activation(inputs[0]) if kept is None else kept)
             else:
                 layer.acts.append(inputs[0].detach())
             layer.counter += 1

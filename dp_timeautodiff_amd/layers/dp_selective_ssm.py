@@ -228,7 +228,8 @@ class DPSelectiveSSM(nn.Module):
         return torch.split(dbc, [self.dt_rank, self.state_size, self.state_size], -1)
 
     def forward(self, x, state: Optional[SSMState] = None, lengths=None, return_state: bool = False, kept=None):
-        """x [B,T,d_model]; `kept`: x in 8 bits, if the caller has it (GradSampleModule(activation_bits=8) stashes that)."""
+        """x [B,T,d_model]; `kept`: x in 8 bits, if the caller has it (GradSampleModule(activation_bits=8) stashes that, and refuses
+        one of another shape, dtype or device; that it holds the values of this x is the caller's to see to)."""
         xr, z = torch.split(self.in_proj(x, kept), self.channels, -1)
         conv_state, scan_state = state if state is not None else (None, None)
         u = self.conv(xr, conv_state, lengths, return_state)

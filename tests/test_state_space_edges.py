@@ -288,3 +288,22 @@ def test_removed_hooks_leave_all_layers_to_autograd(dev):
     for n, p in net.named_parameters():
         assert p.grad_sample is None and p.grad is not None, n
         assert float((p.grad.cpu().double() - want[n].sum(0)).abs().max()) <= F32 * x.shape[0] * float(want[n].abs().max()), n
+
+
+def test_an_eight_bit_input_of_another_tensor_is_refused(dev):
+    from dp_timeautodiff_amd.activation8 import compress_activation
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    from dp_timeautodiff_amd.layers import DPSelectiveSSM
+    gsm = GradSampleModule(DPSelectiveSSM(12, 4).to(dev).train(), activation_bits=8)
+    x = torch.randn(3, 5, 12, device=dev)
+    own = compress_activation(x)
+    bad = [compress_activation(x[:, :4]), compress_activation(x.to(torch.bfloat16)), own._replace(exponent=own.exponent[:, :3]),
+           compress_activation(torch.randn(3, 5, 140, device=dev)), own.data]
+    if dev.type == "cuda":
+        bad.append(own._replace(data=own.data.cpu(), exponent=own.exponent.cpu()))
+    for kept in bad:
+        with pytest.raises(ValueError, match="8 bits"):
+            gsm(x, kept=kept)
+    assert gsm._layers[0].acts == []
+    gsm(x, kept=own).sum().backward()
+    gsm.check_complete()
