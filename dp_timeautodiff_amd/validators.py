@@ -54,7 +54,8 @@ class _RMSNormOutput(DPRMSNorm):
 
 
 def _fixable_rms_norm(m: nn.Module) -> bool:
-    return type(m) is nn.RMSNorm and m.elementwise_affine and len(m.normalized_shape) == 1
+    """A trainable nn.RMSNorm that DPRMSNorm can stand for.  (A frozen one needs no per-sample gradients and stays.)"""
+    return (type(m) is nn.RMSNorm and m.elementwise_affine and m.weight.requires_grad and len(m.normalized_shape) == 1)
 
 
 def _replace(root: nn.Module, name: str, new: nn.Module) -> nn.Module:

@@ -307,3 +307,12 @@ def test_an_eight_bit_input_of_another_tensor_is_refused(dev):
     assert gsm._layers[0].acts == []
     gsm(x, kept=own).sum().backward()
     gsm.check_complete()
+
+
+def test_validator_leaves_a_frozen_rms_norm_alone():
+    from dp_timeautodiff_amd.validators import ModuleValidator
+    net = nn.Sequential(nn.Linear(4, 9), nn.RMSNorm(9), nn.Linear(9, 2))
+    net[1].weight.requires_grad_(False)
+    assert ModuleValidator.is_valid(net)
+    fixed = ModuleValidator.fix(net)
+    assert type(fixed[1]) is nn.RMSNorm and not fixed[1].weight.requires_grad and ModuleValidator.is_valid(fixed)
