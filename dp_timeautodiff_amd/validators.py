@@ -18,6 +18,7 @@ from typing import List
 import torch
 import torch.nn as nn
 
+from . import _native
 from .layers import (DPCausalConv, DPGRU, DPLSTM, DPMultiheadAttention, DPRMSNorm, DPSelectiveScan, RNNLinear,
                      SequenceBias)
 
@@ -55,7 +56,8 @@ class _RMSNormOutput(DPRMSNorm):
 
 def _fixable_rms_norm(m: nn.Module) -> bool:
     """A trainable nn.RMSNorm that DPRMSNorm can stand for.  (A frozen one needs no per-sample gradients and stays.)"""
-    return (type(m) is nn.RMSNorm and m.elementwise_affine and m.weight.requires_grad and len(m.normalized_shape) == 1)
+    return (type(m) is nn.RMSNorm and m.elementwise_affine and m.weight.requires_grad and len(m.normalized_shape) == 1
+            and 1 <= m.normalized_shape[0] <= _native.RMS_MAX_FEATURES)
 
 
 def _replace(root: nn.Module, name: str, new: nn.Module) -> nn.Module:

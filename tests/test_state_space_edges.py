@@ -316,3 +316,10 @@ def test_validator_leaves_a_frozen_rms_norm_alone():
     assert ModuleValidator.is_valid(net)
     fixed = ModuleValidator.fix(net)
     assert type(fixed[1]) is nn.RMSNorm and not fixed[1].weight.requires_grad and ModuleValidator.is_valid(fixed)
+
+
+def test_validator_reports_a_norm_too_wide_to_replace():
+    from dp_timeautodiff_amd.validators import ModuleValidator
+    net = nn.Sequential(nn.Linear(4, 9), nn.RMSNorm(16385), nn.RMSNorm((3, 4)))
+    fixed = ModuleValidator.fix(net)   # and does not fail over it
+    assert type(fixed[1]) is nn.RMSNorm and len(ModuleValidator.validate(fixed)) == len(ModuleValidator.validate(net)) == 2
