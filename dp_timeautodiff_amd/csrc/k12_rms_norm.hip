@@ -250,6 +250,7 @@ extern "C" int dpk_rms_norm_forward(const void* X, int64_t ld_x, const void* RES
 #define RMS_CALL(T, E, LPR)                                                                                                  \
     {                                                                                                                        \
         constexpr int NT = LPR > 256 ? LPR : 256, RPB = NT / LPR;                                                            \
+        if (!dpk_launchable((rows + RPB - 1) / RPB, NT)) return DPK_ERANGE;                                                  \
         hipLaunchKernelGGL((rms_forward_kernel<T, E, LPR>), dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(NT), 0,           \
                            (hipStream_t)stream, (const T*)X, ld_x, (const T*)RES, ld_res, W, (T*)Y, (T*)R, rstd, Q, QE, rows, \
                            C, eps);                                                                                          \
@@ -279,7 +280,7 @@ extern "C" int dpk_rms_norm_backward(const void* R, int64_t ld_r, const void* RE
     if ((DW && dw_stride < C) || (RES && dtype == DPK_F32)) return DPK_EINVAL;
     if (groups == 0) return DPK_OK;
     if (!W || (rows_per_group > 0 && (!R || !DY || !rstd))) return DPK_EINVAL;
-    if (C > MAX_C || groups * split > 0x7fffffffLL) return DPK_ERANGE;
+    if (C > MAX_C || groups > 0x7fffffffLL || !dpk_launchable(groups * split, C > 256 * 16 ? 1024 : 256)) return DPK_ERANGE;
 #define RMS_GO(T, E, LPR, SUM, HAS_DR)                                                                                           \
     hipLaunchKernelGGL((rms_backward_kernel<T, E, LPR, SUM, HAS_DR>), dim3((unsigned)(groups * split)),                        \
                        dim3(LPR > 256 ? LPR : 256), 0, (hipStream_t)stream, (const T*)R, ld_r, (const T*)RES, ld_res,           \

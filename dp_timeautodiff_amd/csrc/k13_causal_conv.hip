@@ -246,7 +246,7 @@ constexpr int NARROW = 16, WIDE = 64;   // lanes across channels: 64 channels or
 
 int check(int B, int T, int D, int W, int64_t sb, int64_t st) {
     if (B < 0 || T < 0 || D <= 0 || W <= 0 || sb < 0 || st < 0) return DPK_EINVAL;
-    if (W > 4) return DPK_ERANGE;
+    if (W > 4 || T > MAX_DIM || D > MAX_DIM) return DPK_ERANGE;
     return DPK_OK;
 }
 
@@ -287,7 +287,7 @@ extern "C" int dpk_causal_conv_forward(const void* x, int64_t x_sb, int64_t x_st
     const int cgl = D <= NARROW * CV ? NARROW : WIDE;
     a.nct = (D + cgl * CV - 1) / (cgl * CV);
     const int64_t grid = (int64_t)B * a.nseg * a.nct;
-    if (grid > 0x7fffffffLL) return DPK_ERANGE;
+    if (!dpk_launchable(grid, 256)) return DPK_ERANGE;
 #define CALL(WW)                                                                                                             \
     if (cgl == NARROW)                                                                                                       \
         hipLaunchKernelGGL((conv_forward_kernel<E, WW, NARROW>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a); \
@@ -318,7 +318,7 @@ extern "C" int dpk_causal_conv_backward(const void* x, int64_t x_sb, int64_t x_s
     const int cgl = D <= NARROW * CV ? NARROW : WIDE;
     a.nct = (D + cgl * CV - 1) / (cgl * CV);
     const int64_t grid = (int64_t)B * a.nseg * a.nct;
-    if (grid > 0x7fffffffLL) return DPK_ERANGE;
+    if (!dpk_launchable(grid, 256)) return DPK_ERANGE;
 #define CALL(WW)                                                                                                              \
     if (cgl == NARROW)                                                                                                        \
         hipLaunchKernelGGL((conv_backward_kernel<E, WW, NARROW>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a); \
@@ -336,7 +336,7 @@ extern "C" int dpk_causal_conv_step(const void* x, int64_t x_sb, void* state, co
     if (B == 0) return DPK_OK;
     if (!x || !w || !y || (W > 1 && !state)) return DPK_EINVAL;
     const int64_t total = (int64_t)B * D, grid = (total + 255) / 256;
-    if (grid > 0x7fffffffLL) return DPK_ERANGE;
+    if (!dpk_launchable(grid, 256)) return DPK_ERANGE;
 #define CALL(WW)                                                                                                               \
     hipLaunchKernelGGL((conv_step_kernel<E, WW>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const E*)x, x_sb, \
                        (E*)state, w, bias, (E*)y, total, D, silu);

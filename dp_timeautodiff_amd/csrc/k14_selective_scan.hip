@@ -839,6 +839,8 @@ int block_of(int D) { return D > 192 ? 256 : (D + 63) / 64 * 64; }
 // backward: lanes a channel's states lie on, threads of a workgroup, workgroups a row of channels needs
 int lanes_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 int back_block_of(int D, int N) { return block_of(D > 1024 ? 1024 : D * lanes_of(N)); }
+// lanes that share a state where chunks are joined
+int join_lanes(int nchunk) { return nchunk <= JOIN_RUN ? 1 : nchunk <= 2 * JOIN_RUN ? 2 : nchunk <= 4 * JOIN_RUN ? 4 : 8; }
 int back_blocks_of(int D, int N) {
     const int per = back_block_of(D, N) / lanes_of(N);
     return (D + per - 1) / per;
@@ -846,7 +848,7 @@ int back_blocks_of(int D, int N) {
 
 int check(const dpk_scan_desc* s) {
     if (!s || s->B < 0 || s->T < 0 || s->D <= 0 || s->N <= 0) return DPK_EINVAL;
-    if (s->N > DPK_SCAN_MAX_STATE) return DPK_ERANGE;
+    if (s->N > DPK_SCAN_MAX_STATE || s->T > MAX_DIM) return DPK_ERANGE;
     if (s->dtype != DPK_F32 && s->dtype != DPK_BF16 && s->dtype != DPK_F16) return DPK_EINVAL;
     if (s->nchunk <= 0 || s->chunk < 0 || s->chunk % GROUP || (int64_t)s->nchunk * s->chunk < s->T) return DPK_EINVAL;
     if (s->u_sb < 0 || s->u_st < 0 || s->delta_sb < 0 || s->delta_st < 0 || s->B_sb < 0 || s->B_st < 0 || s->C_sb < 0 ||
@@ -858,12 +860,20 @@ int check(const dpk_scan_desc* s) {
         s->z_st >= row_limit || s->B_st >= row_limit || s->C_st >= row_limit)
         return DPK_ERANGE;
     if (!s->A_log || (s->T > 0 && (!s->u || !s->delta || !s->Bm || !s->Cm))) return DPK_EINVAL;
-    const int bl = block_of(s->D);
-    if ((int64_t)s->B * s->nchunk * ((s->D + bl - 1) / bl) > 0x7fffffffLL ||
-        (int64_t)s->B * s->nchunk * back_blocks_of(s->D, s->N) > 0x7fffffffLL)
-        return DPK_ERANGE;
-    if (((int64_t)s->B * s->N * s->D + 31) / 32 > 0x7fffffffLL) return DPK_ERANGE;
     return DPK_OK;
+}
+
+// whether every launch of a direction can be made (looked at before the first one)
+bool launches(const dpk_scan_desc* s, bool backward) {
+    const int64_t runs = (int64_t)s->B * s->nchunk;
+    const int bl = block_of(s->D), back = back_block_of(s->D, s->N), per = 256 / join_lanes(s->nchunk);
+    const int64_t states = (int64_t)s->B * s->N * s->D;
+    if (runs > 0x7fffffffLL) return false;
+    if ((!backward || s->nchunk > 1) && !dpk_launchable(runs * ((s->D + bl - 1) / bl), bl)) return false;
+    if (s->nchunk > 1 && !dpk_launchable((states + per - 1) / per, 256)) return false;
+    if (!backward) return true;
+    const int blocks = back_blocks_of(s->D, s->N);
+    return dpk_launchable(runs * blocks, back) && (blocks == 1 || dpk_launchable(((int64_t)s->B * s->T * 2 * s->N + 255) / 256, 256));
 }
 
 ScanArgs fill(const dpk_scan_desc* s) {
@@ -887,10 +897,12 @@ void join(const ScanArgs& a, hipStream_t st) {
 #define CALL(LANES)                                                                                                             \
     hipLaunchKernelGGL((scan_join_kernel<REVERSE, LANES>), dim3((unsigned)((states + 256 / LANES - 1) / (256 / LANES))), dim3(256), \
                        0, st, a)
-    if (a.nchunk <= JOIN_RUN) CALL(1);
-    else if (a.nchunk <= 2 * JOIN_RUN) CALL(2);
-    else if (a.nchunk <= 4 * JOIN_RUN) CALL(4);
-    else CALL(8);
+    switch (join_lanes(a.nchunk)) {
+        case 1: CALL(1); break;
+        case 2: CALL(2); break;
+        case 4: CALL(4); break;
+        default: CALL(8); break;
+    }
 #undef CALL
 }
 
@@ -939,6 +951,7 @@ extern "C" int dpk_selective_scan_forward(const dpk_scan_desc* s, void* out, flo
     if (s->B == 0) return DPK_OK;
     if (s->T > 0 && !out) return DPK_EINVAL;
     if (s->nchunk > 1 && (!s->edge || !s->span)) return DPK_EINVAL;
+    if (!launches(s, false)) return DPK_ERANGE;
     ScanArgs a = fill(s);
     a.out = out; a.hT = hT;
     const hipStream_t st = (hipStream_t)stream;
@@ -964,6 +977,7 @@ extern "C" int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_sca
     if (s->T > 0 && (!g->dout || !g->du || !g->ddelta || !g->dB || !g->dC || !s->kept || (s->z && !g->dz))) return DPK_EINVAL;
     if (s->nchunk > 1 && (!s->edge || !s->span)) return DPK_EINVAL;
     if ((g->dA || g->dD || g->dbias) && g->par_stride < s->D) return DPK_EINVAL;
+    if (!launches(s, true)) return DPK_ERANGE;
     ScanArgs a = fill(s);
     const int blocks = back_blocks_of(s->D, s->N);
     if (blocks > 1 && s->T > 0 && !g->dbc) return DPK_EINVAL;
@@ -973,7 +987,6 @@ extern "C" int dpk_selective_scan_backward(const dpk_scan_desc* s, const dpk_sca
     const hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)(a.nb * a.nchunk * a.ndb)), block((unsigned)block_of(a.D));
     const int64_t sums = (int64_t)a.nb * a.T * 2 * a.N;
-    if ((sums + 255) / 256 > 0x7fffffffLL) return DPK_ERANGE;
     if (a.nchunk > 1) {
 #define CALL(NT) hipLaunchKernelGGL((scan_backward_edge_kernel<E, NT>), grid, block, 0, st, a);
         DPK_DISPATCH_DTYPE(s->dtype, E, SCAN_N(a.N, CALL))
@@ -1002,7 +1015,7 @@ extern "C" int dpk_selective_scan_step(const dpk_scan_desc* s, float* state, voi
     a.hT = state; a.out = out;
     const int lanes = s->N <= 4 ? 1 : s->N <= 8 ? 2 : s->N <= 16 ? 4 : 8;
     const int64_t grid = ((int64_t)a.nb * a.D * lanes + 255) / 256;
-    if (grid > 0x7fffffffLL) return DPK_ERANGE;
+    if (!dpk_launchable(grid, 256)) return DPK_ERANGE;
 #define CALL(L) hipLaunchKernelGGL((scan_step_kernel<E, L>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
     DPK_DISPATCH_DTYPE(s->dtype, E, if (lanes == 1) { CALL(1) } else if (lanes == 2) { CALL(2) } else if (lanes == 4) { CALL(4) } else { CALL(8) })
 #undef CALL

@@ -197,9 +197,10 @@ extern "C" int dpk_compress_activation(const void* X, int64_t ld_x, int8_t* Q, u
     if (rows < 0 || C <= 0 || ld_x < 0) return DPK_EINVAL;
     if (rows == 0) return DPK_OK;
     if (!X || !Q || !E) return DPK_EINVAL;
+    if (C > MAX_DIM || rows > (int64_t)1 << 36) return DPK_ERANGE;
     const int nb = (C + BLK - 1) / BLK;
     const int64_t total = rows * nb, units = dtype == DPK_F32 ? ShapeOf<float>::UNITS : ShapeOf<__bf16>::UNITS, grid = (total + units - 1) / units;
-    if (rows > (int64_t)1 << 40 || grid > 0x7fffffffLL) return DPK_ERANGE;
+    if (!dpk_launchable(grid, 256)) return DPK_ERANGE;
     DPK_DISPATCH_DTYPE(dtype, T, hipLaunchKernelGGL(compress_kernel<T>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream,
                                                     (const T*)X, ld_x, Q, E, total, C, nb);)
     return dpk_launch_status();
@@ -209,9 +210,10 @@ extern "C" int dpk_restore_activation(const int8_t* Q, const uint8_t* E, void* X
     if (rows < 0 || C <= 0) return DPK_EINVAL;
     if (rows == 0) return DPK_OK;
     if (!X || !Q || !E) return DPK_EINVAL;
+    if (C > MAX_DIM || rows > (int64_t)1 << 36) return DPK_ERANGE;
     const int nb = (C + BLK - 1) / BLK;
     const int64_t total = rows * nb, units = dtype == DPK_F32 ? ShapeOf<float>::UNITS : ShapeOf<__bf16>::UNITS, grid = (total + units - 1) / units;
-    if (rows > (int64_t)1 << 40 || grid > 0x7fffffffLL) return DPK_ERANGE;
+    if (!dpk_launchable(grid, 256)) return DPK_ERANGE;
     DPK_DISPATCH_DTYPE(dtype, T, hipLaunchKernelGGL(restore_kernel<T>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, Q,
                                                     E, (T*)X, total, C, nb);)
     return dpk_launch_status();
@@ -231,7 +233,7 @@ extern "C" int dpk_sum_rows(const float* in, int groups, int rows, int64_t in_st
     if (rows > 0 && !in) return DPK_EINVAL;
     const bool narrow = a.P <= 2048 && rows > 64;
     const int64_t gx = narrow ? (a.P + 15) / 16 : (a.P + 63) / 64;
-    if (gx > 0x7fffffffLL || groups > 65535) return DPK_ERANGE;
+    if (!dpk_launchable(gx, 1024) || groups > 65535) return DPK_ERANGE;
     a.in = in; a.in_stride = in_stride; a.R = rows; a.accumulate = accumulate; a.scale = scale;
     const dim3 grid((unsigned)gx, (unsigned)groups);
     if (narrow)

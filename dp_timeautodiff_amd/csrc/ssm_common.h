@@ -116,6 +116,12 @@ __device__ __forceinline__ int quantize8(float v, float inv, int byte) {
     return (int)__builtin_amdgcn_fmed3f(rintf(v * inv), -top, top);
 }
 
+// A launch counts its threads in 32 bits, and kernels count steps and channels in int with room for a tile past the end.
+static inline bool dpk_launchable(int64_t blocks, int threads) {
+    return blocks <= 0x7fffffffLL && blocks * threads <= 0xffffffffLL;
+}
+constexpr int MAX_DIM = 1 << 30;
+
 #define DPK_DISPATCH_DTYPE(dtype, T, ...)                                   \
     switch (dtype) {                                                        \
         case DPK_F32: { using T = float; __VA_ARGS__ } break;               \

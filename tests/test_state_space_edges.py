@@ -323,3 +323,48 @@ def test_validator_reports_a_norm_too_wide_to_replace():
     net = nn.Sequential(nn.Linear(4, 9), nn.RMSNorm(16385), nn.RMSNorm((3, 4)))
     fixed = ModuleValidator.fix(net)   # and does not fail over it
     assert type(fixed[1]) is nn.RMSNorm and len(ModuleValidator.validate(fixed)) == len(ModuleValidator.validate(net)) == 2
+
+
+# ---- sizes past what a launch can count -------------------------------------------------------------------------------------------------
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """A launch counts its threads in 32 bits.  Every call is refused before anything is launched (no GPU needed)."""
+    from dp_timeautodiff_amd import _native
+    lib = _native.load()
+    p = ctypes.c_void_p(4096)   # never dereferenced
+    norm = lambda rows, C: lib.dpk_rms_norm_forward(p, C, None, 0, p, p, None, None, None, None, rows, C, 1e-6, 0, None)  # noqa: E731
+    # a row takes 32, 64, 256 or 1024 threads
+    assert norm(2 ** 27, 8) == norm(2 ** 26, 200) == norm(2 ** 24, 1025) == norm(2 ** 22, 5000) == -2
+    assert lib.dpk_rms_norm_backward(p, 8, None, 0, p, 8, None, 0, p, p, p, p, 8, 2 ** 24, 4, 1, 8, 1.0, 0, 0, None) == -2
+    assert lib.dpk_rms_norm_backward(p, 8, None, 0, p, 8, None, 0, p, p, p, p, 8, 2 ** 20, 4, 16, 8, 1.0, 0, 0, None) == -2
+    assert lib.dpk_rms_norm_backward(p, 5000, None, 0, p, 5000, None, 0, p, p, p, p, 5000, 2 ** 22, 4, 1, 5000, 1.0, 0, 0, None) == -2
+    conv = lambda B, T, D: lib.dpk_causal_conv_forward(p, 24, 8, p, None, None, None, p, None, B, T, D, 4, 1, 0, None)  # noqa: E731
+    assert conv(2 ** 24, 1, 8) == conv(1, 2 ** 30 + 1, 8) == conv(1, 4, 2 ** 30 + 1) == -2
+    assert lib.dpk_causal_conv_backward(p, 24, 8, p, 24, 8, p, None, None, None, None, p, None, None, 0, -1, 1, 2 ** 24, 1, 8, 4, 1, 1.0, 0, 0,
+                                        None) == -2
+    assert lib.dpk_causal_conv_step(p, 2 ** 20, p, p, None, p, 2 ** 12, 2 ** 20, 4, 1, 0, None) == -2
+
+    def scan(**k):
+        s = _native._ScanDesc()
+        for n, v in dict(dict(B=2, T=8, D=8, N=4, dtype=0, nchunk=1, chunk=8, u=4096, delta=4096, Bm=4096, Cm=4096, A_log=4096, kept=4096,
+                              edge=4096, span=4096), **k).items():
+            setattr(s, n, v)
+        return s
+
+    g = _native._ScanGrads()
+    for n in ("dout", "du", "ddelta", "dB", "dC", "dbc"):
+        setattr(g, n, 4096)
+    fwd = lambda **k: lib.dpk_selective_scan_forward(ctypes.byref(scan(**k)), p, None, None)  # noqa: E731
+    back = lambda **k: lib.dpk_selective_scan_backward(ctypes.byref(scan(**k)), ctypes.byref(g), None)  # noqa: E731
+    assert fwd(B=2 ** 26) == back(B=2 ** 26) == fwd(B=2 ** 24, D=256) == fwd(T=2 ** 30 + 1, chunk=2 ** 30 + 8) == -2
+    assert back(B=2 ** 22, D=256, N=16) == -2                                        # four workgroups of 256 threads a sequence
+    assert fwd(B=2 ** 22, T=24, nchunk=16, chunk=8) == -2                            # 64 threads a chunk
+    assert fwd(B=2 ** 20, T=64 * 33, nchunk=33, chunk=64, D=64, N=32) == -2          # chunks, and eight lanes a state to join them
+    assert back(B=2 ** 20, T=2 ** 12, chunk=2 ** 12, D=300) == -2                    # 2^32 sums over channel blocks and more
+    step = lambda **k: lib.dpk_selective_scan_step(ctypes.byref(scan(T=1, **k)), p, p, None)  # noqa: E731
+    assert step(B=2 ** 20, D=2 ** 12) == step(B=2 ** 20, D=2 ** 10, N=16) == -2
+    assert lib.dpk_compress_activation(p, 1, p, p, 2 ** 29 + 1, 1, 0, None) == lib.dpk_restore_activation(p, p, p, 2 ** 29 + 1, 1, 0, None) == -2
+    assert lib.dpk_compress_activation(p, 2 ** 31 - 1, p, p, 1, 2 ** 31 - 1, 0, None) == -2
+    out, n, st = (ctypes.c_void_p * 3)(4096, None, None), (ctypes.c_int64 * 3)(2 ** 29, 0, 0), (ctypes.c_int64 * 3)(2 ** 29, 0, 0)
+    assert lib.dpk_sum_rows(p, 1, 4, 2 ** 29, out, n, st, 1.0, 0, None) == -2
