@@ -669,6 +669,7 @@ RMS_MAX_FEATURES = 16384
 CONV_MAX_WIDTH = 4
 SCAN_MAX_STATE = 32
 ACT8_BLOCK = 128
+MAX_DIM = 1 << 30
 
 
 def _act(t, name: str, shape=None, like: Optional[torch.Tensor] = None):
@@ -696,6 +697,12 @@ def _par(t, name: str, shape, device, dtype=torch.float32):
     if tuple(t.shape) != tuple(shape) or t.device != device:
         raise DpkError(f"{name}: expected shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
     return _dense(t)
+
+
+def _dims(name: str, *sizes):
+    """Sizes that go to the library as C ints, of which ctypes would keep the low 32 bits without a word."""
+    if max(sizes) > MAX_DIM:
+        raise DpkError(f"{name}: at most {MAX_DIM} along a dimension, got {max(sizes)}")
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent in builds of torch without a GPU runtime
@@ -819,6 +826,7 @@ def _conv_args(x, weight, bias, state, lengths):
     if x.dim() != 3 or x.shape[2] == 0:
         raise DpkError(f"causal_conv: x must be [B, T, D] with D > 0, got {tuple(x.shape)}")
     B, T, D = x.shape
+    _dims("causal_conv", B, T, D)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= CONV_MAX_WIDTH:
         raise DpkError(f"causal_conv: weight must be [D, W] with W of 1 to {CONV_MAX_WIDTH}")
     W = weight.shape[1]
@@ -894,6 +902,7 @@ def causal_conv_step(x, state, weight, bias, silu: bool):
     if x.dim() != 2 or x.shape[1] == 0:
         raise DpkError(f"causal_conv_step: x must be [B, D] with D > 0, got {tuple(x.shape)}")
     B, D = x.shape
+    _dims("causal_conv_step", B, D)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= CONV_MAX_WIDTH:
         raise DpkError(f"causal_conv_step: weight must be [D, W] with W of 1 to {CONV_MAX_WIDTH}")
     W = weight.shape[1]
@@ -935,6 +944,7 @@ class ScanInputs:
             raise DpkError(f"selective_scan: u must be {'[B, D]' if step else '[B, T, D]'} with D > 0, got {tuple(u.shape)}")
         if not isinstance(A_log, torch.Tensor) or A_log.dim() != 2 or not 1 <= A_log.shape[1] <= SCAN_MAX_STATE:
             raise DpkError(f"selective_scan: A_log must be [D, N] with N of 1 to {SCAN_MAX_STATE}")
+        _dims("selective_scan", *u.shape)
         d, n = u.shape[-1], A_log.shape[1]
         rows = tuple(u.shape[:-1])
         _act(delta, "delta", u.shape, u)
@@ -1076,6 +1086,7 @@ def compress_activation(x):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise DpkError("compress_activation: expected [..., C] with C > 0")
     C = x.shape[-1]
+    _dims("compress_activation", C)
     x, ld = _as_rows(x)
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     e = torch.empty(*x.shape[:-1], -(-C // ACT8_BLOCK), dtype=torch.uint8, device=x.device)
@@ -1090,6 +1101,7 @@ def restore_activation(q, e, dtype):
     if dtype not in ACT_DTYPES:
         raise DpkError(f"restore_activation: expected fp32, bf16 or fp16, got {dtype}")
     C = q.shape[-1]
+    _dims("restore_activation", C)
     if tuple(e.shape) != tuple(q.shape[:-1]) + (-(-C // ACT8_BLOCK),) or e.device != q.device:
         raise DpkError("restore_activation: data and exponents do not belong together")
     if not q.is_contiguous() or not e.is_contiguous():

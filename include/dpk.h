@@ -328,8 +328,8 @@ int dpk_adam_step(const float* grad, float* exp_avg, float* exp_avg_sq, const in
  * activations held in 8 bits.  No counterpart in the reference, whose sequence layers are recurrences (K8, K10): these are the
  * same step of a DP-SGD pass for a layer whose recurrence is elementwise.  Activations are fp32, bf16 or fp16 (`dtype`), read at
  * element alignment through element strides (last dimension contiguous) and written contiguous; parameters, their gradients,
- * states of the scan and all sums are fp32.  Every sum has a fixed order.  What would take a launch of 2^32 threads or more, or has
- * 2^30 steps or channels and more, is refused with DPK_ERANGE before anything is launched.
+ * states of the scan and all sums are fp32.  Every sum has a fixed order.  What would take a launch of 2^32 threads, or has
+ * more than 2^30 steps or channels, is refused with DPK_ERANGE before anything is launched.
  */
 #define DPK_F32 0
 #define DPK_BF16 1

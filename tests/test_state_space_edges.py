@@ -368,3 +368,23 @@ def test_launches_of_too_many_threads_are_refused():
     assert lib.dpk_compress_activation(p, 2 ** 31 - 1, p, p, 1, 2 ** 31 - 1, 0, None) == -2
     out, n, st = (ctypes.c_void_p * 3)(4096, None, None), (ctypes.c_int64 * 3)(2 ** 29, 0, 0), (ctypes.c_int64 * 3)(2 ** 29, 0, 0)
     assert lib.dpk_sum_rows(p, 1, 4, 2 ** 29, out, n, st, 1.0, 0, None) == -2
+
+
+@pytest.mark.parametrize("size", [2 ** 30 + 1, 2 ** 32 + 3])
+def test_sizes_past_a_c_int_are_refused(monkeypatch, size):
+    """(The tensors are one element seen over and over; ctypes would pass 2^32 + 3 on as 3.)"""
+    from dp_timeautodiff_amd import _native
+    monkeypatch.setattr(_native, "_act", lambda *a: None)
+    monkeypatch.setattr(_native, "_req", lambda *a: None)
+    one = torch.zeros(1)
+    wide = lambda *s, dtype=torch.float32: one.to(dtype).expand(*s)  # noqa: E731
+    for call in (lambda: _native._conv_args(wide(1, size, 1), one.view(1, 1), None, None, None),
+                 lambda: _native._conv_args(wide(size, 1, 1), one.view(1, 1), None, None, None),
+                 lambda: _native._conv_args(wide(1, 1, size), wide(size, 1), None, None, None),
+                 lambda: _native.causal_conv_step(wide(size, 1), wide(size, 0, 1), one.view(1, 1), None, True),
+                 lambda: _native.ScanInputs(wide(1, size, 1), wide(1, size, 1), one.view(1, 1), wide(1, size, 1), wide(1, size, 1), *[None] * 5, True),
+                 lambda: _native.ScanInputs(wide(size, 1), wide(size, 1), one.view(1, 1), wide(size, 1), wide(size, 1), *[None] * 5, True, step=True),
+                 lambda: _native.compress_activation(wide(size)), lambda: _native.compress_activation(wide(2, size)),
+                 lambda: _native.restore_activation(wide(1, size, dtype=torch.int8), wide(1, -(-size // 128), dtype=torch.uint8), torch.float32)):
+        with pytest.raises(_native.DpkError, match="along a dimension"):
+            call()
