@@ -388,3 +388,67 @@ def test_sizes_past_a_c_int_are_refused(monkeypatch, size):
                  lambda: _native.restore_activation(wide(1, size, dtype=torch.int8), wide(1, -(-size // 128), dtype=torch.uint8), torch.float32)):
         with pytest.raises(_native.DpkError, match="along a dimension"):
             call()
+
+
+# ---- rows spread over several waves, many to a workgroup ----------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,C", [(4200, 600), (4200, 1025), (4200, 2100), (2100, 4100)])
+def test_wide_norms_over_many_rows(dtype, rows, C):
+    """From 513 (16 bits) or 1025 features on, four or sixteen waves share a row and meet in LDS; here every workgroup of the backward
+    pass goes through that at least four times."""
+    import test_state_space_gpu as G
+    from dp_timeautodiff_amd.layers import rms_norm
+    x, res, dy, dr = G.make(rows + C, dtype, *[(rows, C)] * 4)
+    w, = G.make(1, torch.float32, (C,))
+    x64, r64, w64 = G.leaf64(x, res, w)
+    y_ref, r_ref = R.rms_norm(x64, w64, r64)
+    ((y_ref * dy.double()).sum() + (r_ref * dr.double()).sum()).backward()
+    xg, rg, wg = G.leaf(x, res, w)
+    y, r = rms_norm(xg, wg, rg)
+    torch.autograd.backward((y, r), (dy.cuda(), dr.cuda()))
+    G.close(y, y_ref, "y")
+    G.close(r, r_ref, "r")
+    G.close(xg.grad, x64.grad, "dx")
+    G.close(rg.grad, r64.grad, "dresidual")
+    G.close(wg.grad, w64.grad, "dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [1025, 2049, 4100])
+def test_wide_norms_per_sample(C):
+    """Seven rows of one sample to a workgroup."""
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    from dp_timeautodiff_amd.layers import DPRMSNorm
+    B, T = 600, 7
+    g = torch.Generator().manual_seed(C)
+    x, dy = torch.randn(B, T, C, generator=g), torch.randn(B, T, C, generator=g)
+    norm = DPRMSNorm(C).cuda().train()
+    with torch.no_grad():
+        norm.weight.copy_(torch.rand(C, generator=g) + 0.5)
+    gsm = GradSampleModule(norm, loss_reduction="sum")
+    xg = x.cuda().requires_grad_()
+    gsm(xg)[0].backward(dy.cuda())
+    gsm.check_complete()
+    x64 = x.double().requires_grad_()
+    y, _ = R.rms_norm(x64, norm.weight.detach().cpu().double())
+    (y * dy.double()).sum().backward()
+    want = (dy.double() * (y.detach() / norm.weight.detach().cpu().double())).sum(1)
+    got = norm.weight.grad_sample.cpu().double()
+    assert got.shape == want.shape and float((got - want).abs().max()) <= F32 * float(want.abs().max())
+    assert float((xg.grad.cpu().double() - x64.grad).abs().max()) <= F32 * float(x64.grad.abs().max())
+
+
+@pytest.mark.gpu
+def test_grad_samples_on_a_side_stream():
+    """overlap_grad_sample=True: Linear layers write the arena on a stream of their own, the state-space layers on the current one."""
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    net, x, w, want, check = _engine_net(torch.device("cuda:0"))
+    gsm = GradSampleModule(net, loss_reduction="sum", overlap_grad_sample=True)
+    for _ in range(3):
+        gsm.zero_grad()
+        (gsm(x.cuda()) * w.cuda()).sum().backward()
+        gsm.check_complete()
+        check(net, want)
