@@ -181,6 +181,10 @@ class _Layer:
         self.open_task = None  # kind "own": autograd graph task of the backward pass whose rows are being written
 
 
+# what the layers of kind "own" write; a subclass with parameters of its own has no kernel for them
+_OWN_PARAMETERS = {DPRMSNorm: {"weight"}, DPCausalConv: {"weight", "bias"}, DPSelectiveScan: {"A_log", "D", "dt_bias"}}
+
+
 def _kind_of(m: nn.Module) -> Optional[str]:
     t = type(m)
     if t in (nn.Linear, RNNLinear, SSMLinear):
@@ -191,8 +195,9 @@ def _kind_of(m: nn.Module) -> Optional[str]:
         return "layernorm"
     if t is SequenceBias:
         return "seqbias"
-    if issubclass(t, (DPRMSNorm, DPCausalConv, DPSelectiveScan)):
-        return "own"  # the layer's backward kernel writes the per-sample gradients itself
+    for base, names in _OWN_PARAMETERS.items():
+        if issubclass(t, base) and {n for n, _ in m.named_parameters(recurse=False)} <= names:
+            return "own"  # the layer's backward kernel writes the per-sample gradients itself
     return None
 
 

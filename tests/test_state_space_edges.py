@@ -452,3 +452,27 @@ def test_grad_samples_on_a_side_stream():
         (gsm(x.cuda()) * w.cuda()).sum().backward()
         gsm.check_complete()
         check(net, want)
+
+
+# ---- parameters that no kernel, or more than one layer, would write -----------------------------------------------------------------------
+
+
+def test_a_subclass_with_a_parameter_of_its_own_is_refused(dev):
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    from dp_timeautodiff_amd.layers import DPCausalConv, DPRMSNorm, DPSelectiveScan
+
+    def more(base):
+        class More(base):
+            def __init__(self, *a):
+                super().__init__(*a)
+                self.shift = nn.Parameter(torch.zeros(4))
+        return More(4)
+
+    class Renamed(DPRMSNorm):
+        pass
+
+    for base in (DPRMSNorm, DPCausalConv, DPSelectiveScan):
+        with pytest.raises(NotImplementedError):
+            GradSampleModule(more(base).to(dev))
+    GradSampleModule(Renamed(4).to(dev))
+    GradSampleModule(DPCausalConv(4, bias=False).to(dev))
