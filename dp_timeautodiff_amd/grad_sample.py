@@ -334,7 +334,7 @@ class GradSampleModule(nn.Module):
         # anchor of _GradTap (not a parameter: invisible to state_dict / optimizers)
         object.__setattr__(self, "_tap", torch.zeros((), device=device, requires_grad=True))
 
-        covered = set()
+        covered = {}
         for name, sub in m.named_modules():
             own = [p for p in sub.parameters(recurse=False) if p.requires_grad]
             if not own:
@@ -358,10 +358,15 @@ class GradSampleModule(nn.Module):
                 n = 1
             if any(not p.requires_grad for p in sub.parameters(recurse=False)):
                 raise NotImplementedError(f"{name}: partially frozen layers are not supported")
+            for p in own:
+                other = covered.get(id(p))
+                if other is not None and "own" in (kind, other.kind):
+                    raise NotImplementedError(f"{name}: a parameter shared with {other.name} is not supported (each layer writes its "
+                                              "per-sample gradients; share the layer instead)")
             layer = _Layer(name, sub, kind, self.arena.reserve_slots(n), n)
             self._layers.append(layer)
             for p in own:
-                covered.add(id(p))
+                covered[id(p)] = layer
             if kind == "own":
                 object.__setattr__(sub, "_dpk_claim", _Claim(self, layer))
                 continue

@@ -476,3 +476,17 @@ def test_a_subclass_with_a_parameter_of_its_own_is_refused(dev):
             GradSampleModule(more(base).to(dev))
     GradSampleModule(Renamed(4).to(dev))
     GradSampleModule(DPCausalConv(4, bias=False).to(dev))
+
+
+def test_a_parameter_of_two_layers_is_refused(dev):
+    """(One layer called twice adds up; two layers with one parameter would each write its rows.)"""
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    from dp_timeautodiff_amd.layers import DPRMSNorm
+    pair = nn.ModuleList([DPRMSNorm(4), DPRMSNorm(4)]).to(dev)
+    pair[1].weight = pair[0].weight
+    with pytest.raises(NotImplementedError, match="shared"):
+        GradSampleModule(pair)
+    mixed = nn.ModuleList([nn.LayerNorm(4), DPRMSNorm(4)]).to(dev)
+    mixed[1].weight = mixed[0].weight
+    with pytest.raises(NotImplementedError, match="shared"):
+        GradSampleModule(mixed)
