@@ -368,8 +368,7 @@ class GradSampleModule(nn.Module):
             for p in own:
                 covered[id(p)] = layer
             if kind == "own":
-                object.__setattr__(sub, "_dpk_claim", _Claim(self, layer))
-                continue
+                continue  # claimed below, once nothing can be refused any more
             self._handles.append(sub.register_forward_pre_hook(self._make_pre(layer)))
             self._handles.append(sub.register_forward_hook(self._make_fwd(layer)))
             self._handles.append(sub.register_full_backward_hook(self._make_bwd(layer)))
@@ -396,6 +395,9 @@ class GradSampleModule(nn.Module):
             p._dpk_arena = self.arena
             if id(p) not in covered and strict:
                 raise NotImplementedError(f"parameter {n_} is owned by a module without a per-sample-gradient kernel")
+        for layer in self._layers:
+            if layer.kind == "own":
+                object.__setattr__(layer.module, "_dpk_claim", _Claim(self, layer))
 
     # ---- nn.Module plumbing -------------------------------------------------------------------------
     def forward(self, *args, **kwargs):

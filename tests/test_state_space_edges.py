@@ -490,3 +490,14 @@ def test_a_parameter_of_two_layers_is_refused(dev):
     mixed[1].weight = mixed[0].weight
     with pytest.raises(NotImplementedError, match="shared"):
         GradSampleModule(mixed)
+
+
+def test_a_refused_model_keeps_its_layers_to_itself(dev):
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    from dp_timeautodiff_amd.layers import DPRMSNorm
+    net = nn.ModuleDict({"norm": DPRMSNorm(4), "table": nn.Embedding(5, 4, padding_idx=0)}).to(dev)
+    with pytest.raises(NotImplementedError):
+        GradSampleModule(net)
+    x = torch.randn(3, 2, 4, device=dev)
+    net["norm"](x)[0].sum().backward()
+    assert net["norm"].weight.grad is not None and net["norm"]._dpk_claim is None
