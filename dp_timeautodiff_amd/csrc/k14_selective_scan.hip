@@ -645,7 +645,6 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
         const int64_t out_at = (int64_t)t0 * a.D * (int64_t)sizeof(T);
         fetch_bc<T, NT>(a, rb, rc, next, end, nbc);
         {
-        {
             float xs[OWN];
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
@@ -739,7 +738,6 @@ __global__ void __launch_bounds__(256, LS >= 4 ? 3 : 2) scan_backward_kernel(Sca
                 put<T>(out_row(du_b, out_at), to + i * out_step, in ? into[i] * dts[i] + skip * gs[i] : 0.f);
                 put<T>(out_row(dd_b, out_at), to + i * out_step, in ? dpre : 0.f);
             }
-        }
         }
         __syncthreads();   // the group's sums are written, the next group's B and C staged
         char* sums = out_row(sums_b, (int64_t)t0 * sum_step);
@@ -915,12 +913,14 @@ void join(const ScanArgs& a, hipStream_t st) {
     else { CALL(32) }
 
 // Chunks of time a scan is cut into.  Cutting costs a second reading of the inputs and most of the arithmetic again, so it has to
-// win a factor of two or three in waves.  Forward into up to 4096 waves (four a SIMD; 1 x 8192 x 1024, N = 16, bf16: 93 us against
-// 100 with 2048) of chunks as short as 32 steps (2 x 4096 x 500: 75 us against 102 with 64), from fewer than 800 (10 x 2000 x 4096
-// bf16, 640 waves: 706 us against 938 in one piece; 16 x 1000 x 4096, 1024 waves: 549 against 491), of short sequences fewer than
-// 512 (50 x 256 x 1024 fp32, 800 waves: 134 against 127).  Backward into up to 2048 of at least 64 steps (145 us against 154 with
-// 32: its waves hold 16 channels, so there are four times as many to begin with) from fewer than 512 (8 x 1000 x 4096: 690 us
-// against 643).
+// win a factor of two or three in waves.  Times of whole calls at N = 16, bf16 where no type is named.  Forward into up to 4096 waves
+// (four a SIMD; 1 x 8192 x 1024: 87 us, 86 with 2048, 3520 in one piece) of chunks as short as 32 steps (2 x 4096 x 500: 53 us, 65
+// with 64), from fewer than 800 (10 x 2000 x 4096, 640 waves: 606 us, 919 in one piece; 16 x 1000 x 4096, 1024 waves: 467 in one
+// piece, 457 in four), of short sequences fewer than 512 (50 x 256 x 1024 fp32, 800 waves: 120 in one piece, 127 in five).
+// Backward into up to 2048 of at least 64 steps (1 x 8192 x 1024: 203 us, 213 with 32; 2 x 4096 x 500: 131, 120 with 32) from
+// fewer than 512 (8 x 1000 x 4096: 783 us in one piece, 756 in four).  The backward numbers are those of N from 9 to 16, whose waves
+// hold 16 channels; the rule does not go by N, and is off where they hold 64 (N = 4, 8 x 2000 x 4096: 1556 us in one piece, as it says,
+// 657 in four) or 8 (N = 32, 4 x 2000 x 4096: 1994 us in eight, as it says, 1299 in one).
 extern "C" int dpk_selective_scan_chunks(int B, int T, int D, int backward, int* chunk) {
     if (B <= 0 || T <= 0 || D <= 0) {
         if (chunk) *chunk = (T > 0 ? (T + GROUP - 1) / GROUP * GROUP : 0);

@@ -59,7 +59,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     """x [..., C] fp32, bf16 or fp16, residual of the same shape and dtype (or None), weight [C] fp32.
 
     Returns (y, r) with r = x + residual (x itself without a residual), or (y, r, Activation8) with `quantize`: y also in 8
-    bits, as compress_activation would hold it, without reading y again.  The 8-bit form takes no part in autograd."""
+    bits, without reading y again: in fp32 as compress_activation would hold it, in 16 bits from y before its rounding to them.  The
+    8-bit form takes no part in autograd."""
     sink, anchor = _sink if _sink is not None else (None, None)
     if _wants_autograd(anchor, x, residual, weight):
         out = _RMSNorm.apply(x, residual, weight, eps, quantize, sink, anchor)

@@ -338,7 +338,7 @@ int dpk_adam_step(const float* grad, float* exp_avg, float* exp_avg_sq, const in
 /*
  * K12: r = X + RES (RES NULL: r = X and R is not needed), rstd = 1/sqrt(mean_c r^2 + eps), Y = r * rstd * W over rows of C <=
  * 16384 elements.  R, rstd (rows floats) may be NULL.  Q [rows, C] and QE [rows, ceil(C/128)] (both or neither) receive Y in 8 bits, as
- * dpk_compress_activation would hold it.
+ * dpk_compress_activation holds it, but from the fp32 values (in 16 bits Y is rounded, Q is not twice).
  * backward: DX (nullable) = rstd * (g - xhat * mean_c(g * xhat)) + DR (nullable), g = DY * W, xhat = (R + RES) * rstd: R and RES are
  * forward's X and RES in 16 bits (where its R is the rounded sum), or R and NULL.  The rows are `groups` groups of rows_per_group; DW (nullable) row (group * split + k) receives scale * sum of DY * xhat over the k-th of `split` parts of
  * the group's rows (accumulate: is added to).  dpk_rms_norm_split says how many parts fill the chip; dpk_sum_rows joins them.
