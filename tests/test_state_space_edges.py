@@ -501,3 +501,45 @@ def test_a_refused_model_keeps_its_layers_to_itself(dev):
     x = torch.randn(3, 2, 4, device=dev)
     net["norm"](x)[0].sum().backward()
     assert net["norm"].weight.grad is not None and net["norm"]._dpk_claim is None
+
+
+# ---- the same tensor twice, and nothing at all --------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_one_tensor_as_several_operands():
+    import test_state_space_gpu as G
+    from dp_timeautodiff_amd.layers import rms_norm, selective_scan
+    x, dy, dr, bc = G.make(3, torch.float32, (3, 7, 20), (3, 7, 20), (3, 7, 20), (3, 7, 20))
+    w, a = G.make(4, torch.float32, (20,), (20, 20))
+    (xg, wg), (x64, w64) = G.leaf(x, w), G.leaf64(x, w)
+    y, r = rms_norm(xg, wg, xg)
+    y_ref, r_ref = R.rms_norm(x64, w64, x64)
+    torch.autograd.backward((y, r), (dy.cuda(), dr.cuda()))
+    ((y_ref * dy.double()).sum() + (r_ref * dr.double()).sum()).backward()
+    G.close(xg.grad, x64.grad, "dx")
+    G.close(wg.grad, w64.grad, "dw")
+    # u, delta and z are one tensor, B and C another: its gradient is the sum of theirs, each within F32 of its largest value
+    xg, bg, ag = G.leaf(x, bc, a)
+    parts = G.leaf64(x, x, a, bc, bc, x)
+    ref = R.selective_scan(*parts[:5], None, parts[5])[0]
+    out = selective_scan(xg, xg, ag, bg, bg, None, xg)
+    out.backward(dy.cuda())
+    (ref * dy.double()).sum().backward()
+    G.close(out, ref, "out")
+    for n, got, of in (("x", xg, (0, 1, 5)), ("bc", bg, (3, 4)), ("A_log", ag, (2,))):
+        G.close(got.grad, sum(parts[k].grad for k in of), "d" + n, F32 * sum(float(parts[k].grad.abs().max()) for k in of))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("skip", [True, False])
+def test_an_empty_batch(skip):
+    from dp_timeautodiff_amd.grad_sample import GradSampleModule
+    dev = torch.device("cuda:0")
+    net, _, _, _, _ = _engine_net(dev)
+    gsm = GradSampleModule(net, skip_autograd_param_grads=skip)
+    gsm(torch.zeros(0, 5, 5, device=dev)).sum().backward()
+    gsm.check_complete()
+    for n, p in net.named_parameters():
+        assert p.grad_sample.shape[0] == 0, n
+        assert (p.grad is None) if skip else (p.grad is not None and not p.grad.any()), n
